@@ -52,6 +52,10 @@ EXPORTS = [  # every symbol include/hydra_hip.h declares
     "hydra_host_trace", "hydra_host_trace_read", "hydra_device_link",
     "hydra_test_set", "hydra_test_get",
 ]
+OPTIM_EXPORTS = [  # every symbol include/hydra_optim.h declares
+    "hydra_adamw_create", "hydra_adamw_destroy", "hydra_adamw_workspace", "hydra_adamw_grad_norm",
+    "hydra_adamw_step", "hydra_adamw_step_ctrl", "hydra_moments8_encode", "hydra_moments8_decode",
+]
 MEASURE_EXPORTS = ["hydra_set_variant", "hydra_measure_peer_stamps"]  # include/hydra_measure.h
 
 # hydra_opt_t (include/hydra_hip.h): library options, no environment variables
@@ -78,6 +82,25 @@ PEER_HANDLE_BYTES = 128
 PEER_ALGOS = {"peer": 0, "peer2": 1, "peer1": 2, "peer2w": 3}  # AUTO, TWO_SHOT, ONE_SHOT,
 # TWO_SHOT_PUSH (the fold writes the result into every rank's bucket)
 PEER_OPT_TIMEOUT_MS, PEER_OPT_BLOCKS, PEER_OPT_ONE_SHOT_MAX = 1, 2, 3
+
+
+# hydra_adamw_config_t.flags (include/hydra_optim.h)
+ADAMW_MASTER, ADAMW_BUCKET, ADAMW_NORM_ONLY = 1, 2, 4
+
+
+class AdamWTensor(ctypes.Structure):
+    """hydra_adamw_tensor_t (include/hydra_optim.h)."""
+    _fields_ = [("param", ctypes.c_void_p), ("master", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                ("m", ctypes.c_void_p), ("v", ctypes.c_void_p), ("m_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n", ctypes.c_size_t), ("lr_scale", ctypes.c_float),
+                ("weight_decay", ctypes.c_float)]
+
+
+class AdamWConfig(ctypes.Structure):
+    """hydra_adamw_config_t (include/hydra_optim.h)."""
+    _fields_ = [("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32),
+                ("state_dtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+                ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double)]
 
 
 class PlanOp(ctypes.Structure):
@@ -253,6 +276,16 @@ def _declare(L) -> None:
     L.hydra_comm_phases.argtypes = [vp, ctypes.POINTER(CommPhases)]
     L.hydra_test_set.argtypes = [i, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)]
     L.hydra_test_get.argtypes = [i, ctypes.POINTER(ctypes.c_int64)]
+    u64, dbl = ctypes.c_uint64, ctypes.c_double
+    L.hydra_adamw_create.argtypes = [i, ctypes.POINTER(AdamWConfig), ctypes.POINTER(AdamWTensor), sz,
+                                     ctypes.POINTER(vp)]
+    L.hydra_adamw_destroy.argtypes = [vp]
+    L.hydra_adamw_workspace.argtypes = [vp, ctypes.POINTER(sz)]
+    L.hydra_adamw_grad_norm.argtypes = [vp, vp, dbl, dbl, vp, vp, sz, vp]
+    L.hydra_adamw_step.argtypes = [vp, vp, dbl, ctypes.c_int64, dbl, u64, vp]
+    L.hydra_adamw_step_ctrl.argtypes = [vp, vp, vp, u64, vp]
+    L.hydra_moments8_encode.argtypes = [vp, vp, vp, vp, vp, vp, i, sz, vp]
+    L.hydra_moments8_decode.argtypes = [vp, vp, i, vp, vp, vp, vp, sz, vp]
 
 
 def _load(path):

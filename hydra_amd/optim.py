@@ -1,0 +1,291 @@
+"""The optimizer step on a reduced gradient bucket (include/hydra_optim.h).
+
+What a training program does with a bucket once it is allreduced, on the device and on torch's
+current stream: the norm of all gradients with the clip factor and the finite check, the AdamW step
+over many tensors in one launch, and the conversion of 8-bit moments.  The reference has no
+counterpart; the formulas and the 8-bit format stand in include/hydra_optim.h.
+
+    plan = AdamW(params, grads, m, v, weight_decay=0.1)         # fp32 moments
+    ctrl = Control(device, lr=3e-4)
+    peer.allreduce_(bucket)                                     # grads are views of the bucket
+    plan.grad_norm_(ctrl, max_norm=1.0, grad_scale=1.0 / world) # norm, clip factor, finite check
+    plan.step_(ctrl=ctrl)                                       # skipped where a gradient overflowed
+
+8-bit moments: uint8 tensors of the params' lengths and moment_scales(n) fp32 scales each,
+zeroed to start with, and a seed that stays the same for the whole training:
+
+    plan = AdamW(params, grads, m8, v8, m_scale=ms, v_scale=vs)
+    plan.step_(lr=3e-4, step=1, seed=1234)
+"""
+from __future__ import annotations
+
+import ctypes
+import sys
+
+from . import _lib
+from ._lib import HydraError, check
+
+_is_finalizing = sys.is_finalizing
+
+MOMENT_BLOCK = 256  # elements that share one scale of an 8-bit moment
+
+
+def moment_scales(n: int) -> int:
+    """Scales of an 8-bit moment of n elements."""
+    return -(-n // MOMENT_BLOCK)
+
+
+def _code(dtype) -> int:
+    import torch
+
+    codes = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
+    try:
+        return codes[dtype]
+    except KeyError:
+        raise HydraError(_lib.ERR_INVALID, f"unsupported dtype {dtype}") from None
+
+
+def _list(x) -> list:
+    import torch
+
+    return [x] if isinstance(x, torch.Tensor) else list(x)
+
+
+def _refuse(msg: str):
+    raise HydraError(_lib.ERR_INVALID, msg)
+
+
+class Control:
+    """hydra_adamw_ctrl_t: 64 bytes on the device that carry a step's scalars from grad_norm_ to
+    step_ without a host round trip.  Its fields are 0-d device tensors: lr and step are set by the
+    program (ctrl.lr.fill_(x)), the others are written by grad_norm_."""
+
+    def __init__(self, device, lr: float = 0.0, step: int = 0):
+        import torch
+
+        self.buffer = torch.zeros(64, dtype=torch.uint8, device=device)
+        if not self.buffer.is_cuda:
+            _refuse("Control: a GPU device is required")
+        f, i = self.buffer.view(torch.float32), self.buffer.view(torch.int32)
+        self.step, self.skipped = self.buffer.view(torch.int64)[:2]
+        self.lr, self.mult, self.norm = f[4], f[5], f[6]
+        self.skip = i[7]
+        self.lr.fill_(lr)
+        self.step.fill_(step)
+
+
+class AdamW:
+    """A plan (hydra_adamw_t): the tensors that are stepped together, laid out once.
+
+    params, grads, m, v: lists of contiguous tensors on one GPU, alike in length; params and grads
+    in fp32, bf16 or fp16, m and v in fp32, or uint8 with m_scale and v_scale (fp32,
+    moment_scales(n) each).  master: fp32 weights beside 16-bit params, which a step then only
+    writes.  weight_decay and lr_scale: a number, or one for each tensor.  params None: a plan for
+    grad_norm_ alone.  bucket: a 1-d tensor whose views the grads are; each call may then name
+    another bucket of that layout (two buckets in turn, one being reduced while the other is
+    stepped).  The plan keeps the tensors alive; a graph that holds its calls does not."""
+
+    def __init__(self, params, grads, m=None, v=None, *, master=None, m_scale=None, v_scale=None,
+                 betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0,
+                 bucket=None):
+        import torch
+
+        self._h = ctypes.c_void_p()
+        grads = _list(grads)
+        if not grads:
+            _refuse("AdamW: no tensors")
+        k, norm_only = len(grads), params is None
+        lists = {"params": params, "m": m, "v": v, "master": master, "m_scale": m_scale,
+                 "v_scale": v_scale}
+        if norm_only and any(x is not None for x in lists.values()):
+            _refuse("AdamW: a plan without params holds gradients alone")
+        if not norm_only and (m is None or v is None):
+            _refuse("AdamW: m and v are required")
+        lists = {name: _list(x) for name, x in lists.items() if x is not None}
+        device = grads[0].device
+        for name, ts in [("grads", grads), *lists.items()]:
+            if len(ts) != k:
+                _refuse(f"AdamW: {len(ts)} {name} for {k} grads")
+            for t in ts:
+                if not t.is_cuda or t.device != device:
+                    _refuse(f"AdamW: {name} must be on one GPU, that of the grads")
+                if not t.is_contiguous():
+                    _refuse(f"AdamW: {name} must be contiguous")
+                if t.dtype != ts[0].dtype:
+                    _refuse(f"AdamW: {name} must share one dtype")
+        eight = not norm_only and lists["m"][0].dtype == torch.uint8
+        if not norm_only:
+            for name in ("m", "v"):
+                if lists[name][0].dtype != (torch.uint8 if eight else torch.float32):
+                    _refuse("AdamW: m and v must both be float32 or both uint8")
+            if eight != ("m_scale" in lists) or eight != ("v_scale" in lists):
+                _refuse("AdamW: m_scale and v_scale belong to uint8 moments, and to them only")
+            for name in ("master", "m_scale", "v_scale"):
+                if name in lists and lists[name][0].dtype != torch.float32:
+                    _refuse(f"AdamW: {name} must be float32")
+        for name, ts in lists.items():
+            for t, g in zip(ts, grads):
+                want = moment_scales(g.numel()) if name.endswith("_scale") else g.numel()
+                if t.numel() != want:
+                    _refuse(f"AdamW: {name} of {t.numel()} elements where {want} are needed")
+        wd = list(weight_decay) if hasattr(weight_decay, "__iter__") else [weight_decay] * k
+        ls = list(lr_scale) if hasattr(lr_scale, "__iter__") else [lr_scale] * k
+        if len(wd) != k or len(ls) != k:
+            _refuse("AdamW: weight_decay and lr_scale: a number, or one for each tensor")
+
+        base = 0
+        self._bucket_bytes = None
+        if bucket is not None:
+            self._check_bucket_tensor(bucket, grads[0])
+            base = bucket.data_ptr()
+            self._bucket_bytes = bucket.numel() * bucket.element_size()
+            for g in grads:
+                end = g.data_ptr() + g.numel() * g.element_size()
+                if g.numel() and not (base <= g.data_ptr() and end <= base + self._bucket_bytes):
+                    _refuse("AdamW: a grad is not a view of the bucket")
+        self.device, self._grad_dtype, self._bucket = device, grads[0].dtype, bucket
+        # what the launches touch; with buckets of the caller's choice, not the first one's views
+        self._keep = [*lists.values(), grads if bucket is None else ()]
+        ptr = lambda name, i: lists[name][i].data_ptr() if name in lists else None  # noqa: E731
+        ts = (_lib.AdamWTensor * k)()
+        for i, g in enumerate(grads):
+            ts[i] = _lib.AdamWTensor(ptr("params", i), ptr("master", i),
+                                     g.data_ptr() - base if g.numel() else 0, ptr("m", i),
+                                     ptr("v", i), ptr("m_scale", i), ptr("v_scale", i), g.numel(),
+                                     ls[i], wd[i])
+        flags = (_lib.ADAMW_MASTER if master is not None else 0) | \
+                (_lib.ADAMW_BUCKET if bucket is not None else 0) | \
+                (_lib.ADAMW_NORM_ONLY if norm_only else 0)
+        cfg = _lib.AdamWConfig(0 if norm_only else _code(lists["params"][0].dtype),
+                               _code(self._grad_dtype),
+                               _lib.UINT8 if eight else _lib.FLOAT32, flags, betas[0], betas[1], eps)
+        L = _lib.lib()
+        check(L.hydra_adamw_create(device.index, ctypes.byref(cfg), ts, k, ctypes.byref(self._h)))
+        size = ctypes.c_size_t()
+        check(L.hydra_adamw_workspace(self._h, ctypes.byref(size)))
+        self._workspace = size.value
+
+    @staticmethod
+    def _check_bucket_tensor(b, like):
+        if not b.is_cuda or b.device != like.device or b.dtype != like.dtype or b.dim() != 1 or \
+                not b.is_contiguous():
+            _refuse("AdamW: the bucket must be a contiguous 1-d tensor like the grads")
+
+    def _bucket_ptr(self, bucket):
+        if self._bucket is None:
+            if bucket is not None:
+                _refuse("AdamW: the plan was made without a bucket")
+            return None
+        if bucket is None:
+            return self._bucket.data_ptr()
+        self._check_bucket_tensor(bucket, self._bucket)
+        if bucket.numel() * bucket.element_size() < self._bucket_bytes:
+            _refuse("AdamW: the bucket is shorter than the plan's")
+        return bucket.data_ptr()
+
+    def _handle(self):
+        if not self._h:
+            _refuse("AdamW: the plan is closed")
+        return self._h
+
+    def grad_norm_(self, ctrl: Control, max_norm: float = 0.0, grad_scale: float = 1.0, bucket=None,
+                   stream: int | None = None) -> None:
+        """hydra_adamw_grad_norm: norm, clip factor and finite check of all gradients into ctrl, and
+        the next step's number.  max_norm 0: no clipping."""
+        import torch
+
+        h, b = self._handle(), self._bucket_ptr(bucket)
+        if ctrl.buffer.device != self.device:
+            _refuse("grad_norm_: ctrl is on another device")
+        with torch.cuda.device(self.device):
+            s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
+            ws = torch.empty(self._workspace, dtype=torch.uint8, device=self.device)
+            if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
+                ws.record_stream(torch.cuda.ExternalStream(stream))
+            check(_lib.lib().hydra_adamw_grad_norm(h, b, grad_scale, max_norm,
+                                                   ctrl.buffer.data_ptr(), ws.data_ptr(),
+                                                   self._workspace, s))
+
+    def step_(self, lr: float | None = None, step: int | None = None, grad_scale: float = 1.0,
+              ctrl: Control | None = None, seed: int = 0, bucket=None,
+              stream: int | None = None) -> None:
+        """One AdamW step in place: with lr and step (1, 2, ...) from the arguments, or with ctrl
+        from the last grad_norm_ on it.  seed: that of the 8-bit moments' rounding (0: to nearest)."""
+        import torch
+
+        h, b = self._handle(), self._bucket_ptr(bucket)
+        s = stream if stream is not None else torch.cuda.current_stream(self.device).cuda_stream
+        if ctrl is not None:
+            if lr is not None or step is not None or grad_scale != 1.0:
+                _refuse("step_: lr, step and grad_scale come from ctrl")
+            if ctrl.buffer.device != self.device:
+                _refuse("step_: ctrl is on another device")
+            check(_lib.lib().hydra_adamw_step_ctrl(h, b, ctrl.buffer.data_ptr(), seed, s))
+            return
+        if lr is None or step is None:
+            _refuse("step_: lr and step, or ctrl")
+        check(_lib.lib().hydra_adamw_step(h, b, lr, step, grad_scale, seed, s))
+
+    def close(self) -> None:
+        """Waits for the device's work, then releases the plan."""
+        if self._h:
+            _lib.lib().hydra_adamw_destroy(self._h)
+            self._h = ctypes.c_void_p()
+            self._keep = []
+
+    def __del__(self):
+        if _is_finalizing():  # no HIP calls while the interpreter is finalizing
+            return
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _moments(m, v, m8, m_scale, v8, v_scale):
+    """Checks a conversion's tensors; (device, dtype code, n, pointers by name)."""
+    import torch
+
+    if m is None and v is None:
+        _refuse("moments8: neither moment given")
+    n = (m if m is not None else v).numel()
+    ptrs, values = {}, [t for t in (m, v) if t is not None]
+    for x, codes, scale, name in ((m, m8, m_scale, "m"), (v, v8, v_scale, "v")):
+        if x is None:
+            if codes is not None or scale is not None:
+                _refuse(f"moments8: codes or scales of {name} without its values")
+            ptrs[name] = (None, None, None)
+            continue
+        if codes is None or scale is None:
+            _refuse(f"moments8: {name} needs its codes and its scales")
+        for t in (x, codes, scale):
+            if not t.is_cuda or t.device != values[0].device or not t.is_contiguous():
+                _refuse("moments8: contiguous tensors on one GPU are required")
+        if codes.dtype != torch.uint8 or scale.dtype != torch.float32 or x.dtype != values[0].dtype:
+            _refuse("moments8: uint8 codes, float32 scales and values of one dtype are required")
+        if x.numel() != n or codes.numel() != n or scale.numel() != moment_scales(n):
+            _refuse(f"moments8: {name}: lengths do not fit {n} elements")
+        ptrs[name] = (x.data_ptr(), codes.data_ptr(), scale.data_ptr())
+    return values[0].device, _code(values[0].dtype), n, ptrs
+
+
+def moments8_encode_(m8, m_scale, v8, v_scale, m, v, stream: int | None = None) -> None:
+    """One tensor's moments (fp32 or bf16) into 8 bits, to nearest; either moment may be None."""
+    import torch
+
+    dev, code, n, p = _moments(m, v, m8, m_scale, v8, v_scale)
+    with torch.cuda.device(dev):
+        s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
+        check(_lib.lib().hydra_moments8_encode(p["m"][1], p["m"][2], p["v"][1], p["v"][2],
+                                               p["m"][0], p["v"][0], code, n, s))
+
+
+def moments8_decode_(m, v, m8, m_scale, v8, v_scale, stream: int | None = None) -> None:
+    """The values that 8-bit moments stand for, into fp32 or bf16; either moment may be None."""
+    import torch
+
+    dev, code, n, p = _moments(m, v, m8, m_scale, v8, v_scale)
+    with torch.cuda.device(dev):
+        s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
+        check(_lib.lib().hydra_moments8_decode(p["m"][0], p["v"][0], code, p["m"][1], p["m"][2],
+                                               p["v"][1], p["v"][2], n, s))

@@ -68,7 +68,13 @@ __device__ __forceinline__ uint16_t f16op(uint16_t L, uint16_t R, uint16_t C0) {
   float x = h2f(L), y = h2f(R);
   uint16_t res;
   if (OP == kSum) res = f16_assign(L, f2h(x + y));
-  else if (OP == kProduct) res = f16_assign(L, f2h(x * y));
+  else if (OP == kProduct) {
+    float z = x * y;
+    // the product and its rounding stay two operations: joined, they become v_fma_mixlo_f16 with an
+    // addend of +0, which turns a product of -0 into +0
+    asm("" : "+v"(z));
+    res = f16_assign(L, f2h(z));
+  }
   else if (OP == kMax) res = (x < y) ? R : L;
   else res = (y < x) ? R : L;
   return f16_assign(C0, res);

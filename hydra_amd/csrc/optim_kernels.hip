@@ -9,23 +9,13 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "optim_kernels.h"
 #include "reduce_ops.h"
 
 namespace hydra {
 namespace {
-
-// ---- element types -----------------------------------------------------------------------------
-// IEEE conversions (the reduction's f16_t keeps gloo's store quirk: not wanted here)
-__device__ __forceinline__ float widen(float x) { return x; }
-__device__ __forceinline__ float widen(bf16_t x) { return bf2f(x.x); }
-__device__ __forceinline__ float widen(f16_t x) { return h2f(x.x); }
-__device__ __forceinline__ void narrow(float x, float* out) { *out = x; }
-__device__ __forceinline__ void narrow(float x, bf16_t* out) { out->x = f2bf(x); }
-__device__ __forceinline__ void narrow(float x, f16_t* out) {
-  out->x = __builtin_bit_cast(uint16_t, (_Float16)x);
-}
 
 // ---- 8-bit moments -------------------------------------------------------------------------------
 // The code of t in [0, 1.875] is the top of its fp32 bits once the exponent is rebased to a 4-bit
@@ -65,14 +55,130 @@ __device__ __forceinline__ float decode_v(uint32_t c, float scale) {
   return c == 255u ? INFINITY : root * root;
 }
 
-// the largest of every thread's x (>= 0) over the workgroup
-__device__ __forceinline__ float block_max(float x, float* lds) {
-  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
-  __syncthreads();
+// ---- memory ----------------------------------------------------------------------------------------
+// Global memory by a wave-uniform base and a lane's byte offset.  Pointers that come out of a
+// plan's table have to be said to be global: the compiler cannot see it, and flat accesses would
+// also occupy the LDS counters.
+#define GLOBAL __attribute__((address_space(1)))
+typedef GLOBAL char* gptr;
+__device__ __forceinline__ gptr global(const void* p) { return (gptr)(uint64_t)p; }
+// Four consecutive elements of any alignment (that of the element): tensors are views into buckets.
+// gfx950 runs in unaligned access mode, so these stay single 16-, 8- and 4-byte accesses.
+typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t w4h __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t w1 __attribute__((aligned(1)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+// Nontemporal both ways: a step's state is larger than the caches.  64 Mi fp32: 344 us, against 368
+// with plain stores, 362 with plain loads and 361 with both plain.
+template <typename V>
+__device__ __forceinline__ V ldv(gptr p, uint32_t off) {
+  return __builtin_nontemporal_load((const GLOBAL V*)(p + off));
+}
+template <typename V>
+__device__ __forceinline__ void stv(gptr p, uint32_t off, V x) {
+  __builtin_nontemporal_store(x, (GLOBAL V*)(p + off));
+}
+// x as fp32 rounded it: joined with the operation before it, the conversion to fp16 would become one
+// mixed-precision instruction that rounds once
+__device__ __forceinline__ float settled(float x) {
+  asm("" : "+v"(x));
   return x;
+}
+
+// Element i of a tensor of E, and the four from i on.
+template <typename E> struct At;
+template <> struct At<float> {
+  __device__ __forceinline__ static float load(gptr p, uint32_t i) { return *(const GLOBAL float*)(p + i * 4); }
+  __device__ __forceinline__ static void store(gptr p, uint32_t i, float x) { *(GLOBAL float*)(p + i * 4) = x; }
+  typedef w4 raw;
+  __device__ __forceinline__ static raw load4(gptr p, uint32_t i) { return ldv<w4>(p, i * 4); }
+  __device__ __forceinline__ static f4 wide(raw r) {
+    return f4{bitsf(r[0]), bitsf(r[1]), bitsf(r[2]), bitsf(r[3])};
+  }
+  __device__ __forceinline__ static void store4(gptr p, uint32_t i, f4 x) {
+    stv<w4>(p, i * 4, w4{fbits(x[0]), fbits(x[1]), fbits(x[2]), fbits(x[3])});
+  }
+};
+template <> struct At<bf16_t> {
+  __device__ __forceinline__ static float load(gptr p, uint32_t i) { return bf2f(*(const GLOBAL uint16_t*)(p + i * 2)); }
+  __device__ __forceinline__ static void store(gptr p, uint32_t i, float x) {
+    *(GLOBAL uint16_t*)(p + i * 2) = __builtin_bit_cast(uint16_t, (__bf16)x);
+  }
+  typedef w2 raw;
+  __device__ __forceinline__ static raw load4(gptr p, uint32_t i) { return ldv<w2>(p, i * 2); }
+  __device__ __forceinline__ static f4 wide(raw r) {
+    return f4{bitsf(r[0] << 16), bitsf(r[0] & 0xffff0000u), bitsf(r[1] << 16), bitsf(r[1] & 0xffff0000u)};
+  }
+  __device__ __forceinline__ static void store4(gptr p, uint32_t i, f4 x) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 lo{(__bf16)x[0], (__bf16)x[1]}, hi{(__bf16)x[2], (__bf16)x[3]};
+    stv<w2>(p, i * 2, w2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)});
+  }
+};
+template <> struct At<f16_t> {
+  __device__ __forceinline__ static float load(gptr p, uint32_t i) { return h2f(*(const GLOBAL uint16_t*)(p + i * 2)); }
+  __device__ __forceinline__ static void store(gptr p, uint32_t i, float x) {
+    *(GLOBAL uint16_t*)(p + i * 2) = __builtin_bit_cast(uint16_t, (_Float16)settled(x));
+  }
+  typedef w2 raw;
+  __device__ __forceinline__ static raw load4(gptr p, uint32_t i) { return ldv<w2>(p, i * 2); }
+  __device__ __forceinline__ static f4 wide(raw r) {
+    return f4{h2f((uint16_t)r[0]), h2f((uint16_t)(r[0] >> 16)), h2f((uint16_t)r[1]), h2f((uint16_t)(r[1] >> 16))};
+  }
+  __device__ __forceinline__ static void store4(gptr p, uint32_t i, f4 x) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 lo{(_Float16)settled(x[0]), (_Float16)settled(x[1])};
+    const h2 hi{(_Float16)settled(x[2]), (_Float16)settled(x[3])};
+    stv<w2>(p, i * 2, w2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)});
+  }
+};
+// bytes
+__device__ __forceinline__ uint32_t load_byte(gptr p, uint32_t i) { return *(const GLOBAL uint8_t*)(p + i); }
+__device__ __forceinline__ void store_byte(gptr p, uint32_t i, uint32_t x) { *(GLOBAL uint8_t*)(p + i) = (uint8_t)x; }
+// the first `count` (0 to 4) of four
+template <typename E>
+__device__ __forceinline__ f4 load_upto4(gptr p, uint32_t i, uint32_t count) {
+  if (count >= 4) return At<E>::wide(At<E>::load4(p, i));
+  f4 x = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if ((uint32_t)j < count) x[j] = At<E>::load(p, i + j);
+  return x;
+}
+template <typename E>
+__device__ __forceinline__ void store_upto4(gptr p, uint32_t i, f4 x, uint32_t count) {
+  if (count >= 4) {
+    At<E>::store4(p, i, x);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if ((uint32_t)j < count) At<E>::store(p, i + j, x[j]);
+}
+__device__ __forceinline__ uint32_t load_bytes(gptr p, uint32_t i, uint32_t count) {
+  if (count >= 4) return ldv<w1>(p, i);
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if ((uint32_t)j < count) w |= load_byte(p, i + j) << (8 * j);
+  return w;
+}
+__device__ __forceinline__ void store_bytes(gptr p, uint32_t i, uint32_t w, uint32_t count) {
+  if (count >= 4) {
+    stv<w1>(p, i, w);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if ((uint32_t)j < count) store_byte(p, i + j, w >> (8 * j));
+}
+
+// Workgroups are dealt to the 8 XCDs in turn: tile numbers so that each XCD streams one contiguous
+// eighth of the tiles.
+__device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t tiles) {
+  const uint32_t x = b & 7, q = tiles >> 3, r = tiles & 7;
+  return x * q + min(x, r) + (b >> 3);
 }
 
 // ---- AdamW -----------------------------------------------------------------------------------------
@@ -109,63 +215,243 @@ __device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, 
   p = p * k.decay - (m / denom) * k.size;
 }
 
-__device__ __forceinline__ uint32_t random_word(uint64_t i, uint32_t key) {
-  return fmix32(((uint32_t)i * 0x9E3779B1u) ^ ((uint32_t)(i >> 32) * 0x85EBCA6Bu) ^ key);
-}
-
-template <typename P, typename G, bool MASTER, bool S8>
+// fp32 moments: one tile of one tensor per workgroup, 4 elements per lane and turn, the loads of U
+// turns in flight at once.
+#ifndef OPT_U
+#define OPT_U 1
+#endif
+template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
-                                                     const uint32_t* tile_tensor, OptStep st,
-                                                     uint64_t bucket) {
-  const OptTensor T = tensors[tile_tensor[blockIdx.x]];
+                                                     const uint32_t* tile_tensor, uint32_t tiles,
+                                                     OptStep st, uint64_t bucket) {
+  constexpr int U = OPT_U;
+  constexpr uint32_t kTurn = kOptBlock * 4 * U;
+  const uint32_t tile = xcd_tile(blockIdx.x, tiles);
+  const OptTensor T = tensors[tile_tensor[tile]];
   Scalars k;
   if (!load_scalars(st, T, &k)) return;
-  __shared__ float lds[4];
-  const uint64_t base = (uint64_t)(blockIdx.x - T.tile0) * kOptTile;
-  const G* grad = reinterpret_cast<const G*>(bucket + T.grad);
-  P* param = reinterpret_cast<P*>(T.param);
-  for (uint64_t i0 = base; i0 < min(base + kOptTile, T.n); i0 += kOptBlock) {
-    const uint64_t i = i0 + threadIdx.x;
-    const bool on = i < T.n;
-    float p = 0.0f, m = 0.0f, v = 0.0f;
-    if (on) {
-      p = MASTER ? T.master[i] : widen(param[i]);
-      if constexpr (S8) {
-        m = decode_m((uint8_t)T.m[i], T.m_scale[i / kMomentBlock]);
-        v = decode_v((uint8_t)T.v[i], T.v_scale[i / kMomentBlock]);
-      } else {
-        m = reinterpret_cast<const float*>(T.m)[i];
-        v = reinterpret_cast<const float*>(T.v)[i];
-      }
-      adamw(p, widen(grad[i]), m, v, k);
+  const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
+  const uint32_t left = (uint32_t)min(T.n - base, (uint64_t)kOptTile);
+  const gptr grad = global((const void*)(bucket + T.grad)) + base * sizeof(G);
+  const gptr param = global(T.param) + base * sizeof(P), master = global(T.master) + base * 4;
+  const gptr mm = global(T.m) + base * 4, vv = global(T.v) + base * 4;
+  uint32_t i0 = 0;
+  for (; i0 + kTurn <= left; i0 += kTurn) {
+    typename At<P>::raw p[U];
+    typename At<G>::raw g[U];
+    w4 w[U], m[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t i = i0 + (u * kOptBlock + threadIdx.x) * 4;
+      if (MASTER) w[u] = At<float>::load4(master, i);
+      else p[u] = At<P>::load4(param, i);
+      g[u] = At<G>::load4(grad, i);
+      m[u] = At<float>::load4(mm, i);
+      v[u] = At<float>::load4(vv, i);
     }
-    if constexpr (S8) {
-      const float root = sqrtf(v);
-      const float ms = moment_scale(block_max(finite_abs(m), lds));
-      const float vs = moment_scale(block_max(finite_abs(root), lds));
-      if (on) {
-        const uint32_t r = k.stochastic ? random_word(i, k.key) : 0x80008000u;
-        T.m[i] = (char)encode_m(m, moment_inv(ms), r & 0xffffu);
-        T.v[i] = (char)encode_root(root, moment_inv(vs), r >> 16);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t i = i0 + (u * kOptBlock + threadIdx.x) * 4;
+      f4 x = MASTER ? At<float>::wide(w[u]) : At<P>::wide(p[u]);
+      f4 a = At<float>::wide(m[u]), b = At<float>::wide(v[u]);
+      const f4 y = At<G>::wide(g[u]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        float xj = x[j], aj = a[j], bj = b[j];
+        adamw(xj, y[j], aj, bj, k);
+        x[j] = xj, a[j] = aj, b[j] = bj;
       }
-      if (threadIdx.x == 0) {
-        T.m_scale[i / kMomentBlock] = ms;
-        T.v_scale[i / kMomentBlock] = vs;
-      }
-    } else if (on) {
-      reinterpret_cast<float*>(T.m)[i] = m;
-      reinterpret_cast<float*>(T.v)[i] = v;
+      if (MASTER) At<float>::store4(master, i, x);
+      At<P>::store4(param, i, x);
+      At<float>::store4(mm, i, a);
+      At<float>::store4(vv, i, b);
     }
-    if (on) {
-      if constexpr (MASTER) T.master[i] = p;
-      narrow(p, &param[i]);
+  }
+  for (uint32_t i = i0 + threadIdx.x; i < left; i += kOptBlock) {  // the tensor's last elements
+    float p = MASTER ? At<float>::load(master, i) : At<P>::load(param, i);
+    float m = At<float>::load(mm, i), v = At<float>::load(vv, i);
+    adamw(p, At<G>::load(grad, i), m, v, k);
+    At<float>::store(mm, i, m);
+    At<float>::store(vv, i, v);
+    if (MASTER) At<float>::store(master, i, p);
+    At<P>::store(param, i, p);
+  }
+}
+
+// 8-bit moments: a wave takes one block of 256 elements per turn, 4 per lane, so a block's scales
+// are wave-uniform.
+__device__ __forceinline__ uint32_t wave_umax_pair(uint32_t a, uint32_t b) {
+  // lanes 0-31: a over the wave's halves, lanes 32-63: b; then within 32 lanes, into lanes 31, 63
+  const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  uint32_t x = max((uint32_t)s[0], (uint32_t)s[1]);
+#define HYDRA_DPP_MAX(ctrl) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true))
+  HYDRA_DPP_MAX(0x111);  // row_shr:1
+  HYDRA_DPP_MAX(0x112);
+  HYDRA_DPP_MAX(0x114);
+  HYDRA_DPP_MAX(0x118);
+  HYDRA_DPP_MAX(0x142);  // row_bcast:15
+#undef HYDRA_DPP_MAX
+  return x;
+}
+// c + (low / high half of r) * 16 or * 8: the 16 random bits at the top of what the cut drops
+__device__ __forceinline__ uint32_t add_low16(uint32_t c, uint32_t r) {
+  uint32_t d;
+  asm("v_mad_u32_u16 %0, %1, 16, %2" : "=v"(d) : "v"(r), "v"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t add_high16(uint32_t c, uint32_t r) {
+  uint32_t d;
+  asm("v_mad_u32_u16 %0, %1, 8, %2 op_sel:[1,0,0,0]" : "=v"(d) : "v"(r), "v"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t zero_bytes(uint32_t x) {  // not 0 where x has a byte of 0
+  return (x - 0x01010101u) & ~x & 0x80808080u;
+}
+__device__ __forceinline__ float uniform(float x, int lane) {
+  return bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(x), lane));
+}
+
+// A block's four elements per lane: decode, step, encode.  FAST needs eps in [2^-40, 2^60].  Its
+// shortcuts: no byte that stands for something not finite and both old scales below 2^15 (so
+// 2^112 * scale is finite: one product per value); sqrt and the reciprocal by the hardware's own
+// instructions (1 ulp; they flush below 2^-126, where eps hides it); and new magnitudes whose
+// largest lie in [2^-44, 2^14) (sqrt v) and below 2^14 (m), so that what sqrt flushed is below a
+// byte's smallest step and 2^-112 / scale is normal.  A block that is outside takes the general
+// code for that half.
+template <typename P, typename G, bool MASTER, bool FAST>
+__device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr m8, gptr v8,
+                                       gptr ms, gptr vs, uint32_t count, uint32_t lane,
+                                       uint32_t rnd, uint32_t rkey, const Scalars& k) {
+  // the pointers are the block's; count: elements from this lane's first one to the tensor's end
+  const uint32_t i = lane * 4;
+  f4 p = MASTER ? load_upto4<float>(master, i, count) : load_upto4<P>(param, i, count);
+  const f4 g = load_upto4<G>(grad, i, count);
+  const uint32_t cm = load_bytes(m8, i, count), cv = load_bytes(v8, i, count);
+  const float ms0 = At<float>::load(ms, 0), vs0 = At<float>::load(vs, 0);
+  f4 m, v, root;
+  bool odd = !FAST || !(ms0 < 0x1p15f && vs0 < 0x1p15f) ||
+             __any((zero_bytes(cm ^ 0x80808080u) | zero_bytes(~cv)) != 0);
+  if (odd) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      m[j] = decode_m((cm >> (8 * j)) & 255u, ms0);
+      v[j] = decode_v((cv >> (8 * j)) & 255u, vs0);
     }
+  } else {
+    const float sm = ms0 * 0x1p112f, sv = vs0 * 0x1p112f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      m[j] = bitsf((uint32_t)((int)(int8_t)(cm >> (8 * j)) << 20) & 0x87f00000u) * sm;
+      const float r0 = bitsf(((cv >> (8 * j)) & 255u) << 19) * sv;
+      v[j] = r0 * r0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if (FAST) {
+      const float y = g[j] * k.mult;
+      m[j] = fmaf(y, k.omb1, m[j] * k.b1);
+      v[j] = fmaf(y * k.omb2, y, v[j] * k.b2);
+      root[j] = __builtin_amdgcn_sqrtf(v[j]);
+      const float denom = fmaf(root[j], k.isb2, k.eps);
+      p[j] = fmaf(m[j] * -k.size, __builtin_amdgcn_rcpf(denom), p[j] * k.decay);
+    } else {
+      float pj = p[j], mj = m[j], vj = v[j];
+      adamw(pj, g[j], mj, vj, k);
+      p[j] = pj, m[j] = mj, v[j] = vj;
+      root[j] = sqrtf(vj);
+    }
+  }
+  const uint32_t am = fbits(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
+  const uint32_t ar = max(max(fbits(root[0]), fbits(root[1])), max(fbits(root[2]), fbits(root[3])));
+  const uint32_t top = wave_umax_pair(am, ar);
+  const uint32_t tm = (uint32_t)__builtin_amdgcn_readlane((int)top, 31);
+  const uint32_t tr = (uint32_t)__builtin_amdgcn_readlane((int)top, 63);
+  float scale, s_m, s_v;
+  uint32_t em[4], ev[4], r[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) r[j] = 0x80008000u;
+  if (k.stochastic) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) r[j] = fmix32((rnd + j * 0x9E3779B1u) ^ rkey);
+  }
+  uint32_t wm, wv;
+  if (!odd && tm < fbits(0x1p14f) && tr - fbits(0x1p-44f) < fbits(0x1p14f) - fbits(0x1p-44f)) {
+    const bool none = top < fbits(kTiny);
+    scale = none ? 0.0f : bitsf(top) * kTop;
+    const float inv = none ? 0.0f : __builtin_amdgcn_rcpf(scale) * 0x1p-112f;
+    const float im = uniform(inv, 31), iv = uniform(inv, 63);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      em[j] = min(add_low16(fbits(fabsf(m[j]) * im), r[j]) >> 20, 127u);
+      const uint32_t c = add_high16(fbits(root[j] * iv), r[j]) >> 19;
+      ev[j] = min(min(max(c, 1u), 254u), fbits(v[j]));  // 0 for v = 0 alone
+    }
+    wm = em[0] | em[1] << 8 | em[2] << 16 | em[3] << 24;
+    wv = ev[0] | ev[1] << 8 | ev[2] << 16 | ev[3] << 24;
+    // the signs, but not of zeros
+    const uint32_t hi = __builtin_amdgcn_perm(fbits(m[3]), fbits(m[2]), 0x07030c0cu) |
+                        __builtin_amdgcn_perm(fbits(m[1]), fbits(m[0]), 0x0c0c0703u);
+    wm |= hi & (wm + 0x7f7f7f7fu) & 0x80808080u;
+  } else {
+    float fm = 0.0f, fr = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (FAST) root[j] = sqrtf(v[j]);
+      fm = fmaxf(fm, finite_abs(m[j]));
+      fr = fmaxf(fr, finite_abs(root[j]));
+    }
+    scale = moment_scale(bitsf(wave_umax_pair(fbits(fm), fbits(fr))));
+    s_m = uniform(scale, 31), s_v = uniform(scale, 63);
+    const float im = moment_inv(s_m), iv = moment_inv(s_v);
+    wm = wv = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      wm |= encode_m(m[j], im, r[j] & 0xffffu) << (8 * j);
+      wv |= encode_root(root[j], iv, r[j] >> 16) << (8 * j);
+    }
+  }
+  if ((lane & 31) == 31) At<float>::store(lane & 32 ? vs : ms, 0, scale);
+  if (MASTER) store_upto4<float>(master, i, p, count);
+  store_upto4<P>(param, i, p, count);
+  store_bytes(m8, i, wm, count);
+  store_bytes(v8, i, wv, count);
+}
+
+template <typename P, typename G, bool MASTER>
+__global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
+                                                      const uint32_t* tile_tensor, uint32_t tiles,
+                                                      OptStep st, uint64_t bucket) {
+  const uint32_t tile = xcd_tile(blockIdx.x, tiles);
+  const OptTensor T = tensors[tile_tensor[tile]];
+  Scalars k;
+  if (!load_scalars(st, T, &k)) return;
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const bool fast = k.eps >= 0x1p-40f && k.eps <= 0x1p60f;
+  const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
+  const uint32_t left = (uint32_t)min(T.n - base, (uint64_t)kOptTile);
+  const uint32_t rlane = lane * 4 * 0x9E3779B1u;
+  for (uint32_t i0 = wave * kMomentBlock; i0 < left; i0 += kOptBlock / 64 * kMomentBlock) {
+    const uint64_t at = base + i0;  // the wave's block
+    const uint32_t count = left - i0 > lane * 4 ? left - i0 - lane * 4 : 0u;
+    const uint32_t rnd = (uint32_t)at * 0x9E3779B1u + rlane;
+    const uint32_t rkey = k.key ^ ((uint32_t)(at >> 32) * 0x85EBCA6Bu);
+    const gptr master = global(T.master) + at * 4, param = global(T.param) + at * sizeof(P);
+    const gptr grad = global((const void*)(bucket + T.grad)) + at * sizeof(G);
+    const gptr m8 = global(T.m) + at, v8 = global(T.v) + at;
+    const gptr ms = global(T.m_scale) + at / kMomentBlock * 4;
+    const gptr vs = global(T.v_scale) + at / kMomentBlock * 4;
+    if (fast)
+      block8<P, G, MASTER, true>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
+    else
+      block8<P, G, MASTER, false>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
   }
 }
 
 // ---- the norm --------------------------------------------------------------------------------------
 // fp64 sums: no gradient's square overflows, and the sum is not finite exactly when some gradient
-// is not.  The order is the grid's, which the plan fixes.
+// is not.  The order is the grid's, which the plan fixes: workgroup b sums a contiguous run of tiles.
 __device__ __forceinline__ double block_sum(double x, double* lds) {
   for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
@@ -173,25 +459,61 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
+#ifndef NORM_U
+#define NORM_U 4
+#endif
+template <typename G> struct Words { typedef w4h type; };  // 16 bytes of gradients
+template <> struct Words<float> { typedef w4 type; };
+// the squares of a dword's gradients
+template <typename G>
+__device__ __forceinline__ void add_squares(uint32_t w, double& sum) {
+  if constexpr (sizeof(G) == 4) {
+    const double g = bitsf(w);
+    sum = fma(g, g, sum);
+  } else {
+    constexpr bool half = std::is_same<G, f16_t>::value;
+    const double a = half ? h2f((uint16_t)w) : bitsf(w << 16);
+    const double b = half ? h2f((uint16_t)(w >> 16)) : bitsf(w & 0xffff0000u);
+    sum = fma(a, a, sum);
+    sum = fma(b, b, sum);
+  }
+}
 template <typename G>
 __global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* tensors,
                                                             const uint32_t* tile_tensor,
                                                             uint32_t tiles, uint64_t bucket,
                                                             double* partials) {
+  constexpr int N = 16 / sizeof(G), U = NORM_U;  // elements of a 16-byte load, loads in flight
+  constexpr uint32_t kTurn = kOptBlock * N * U;
   __shared__ double lds[4];
+  const uint32_t b = xcd_tile(blockIdx.x, gridDim.x);
+  uint32_t tile = (uint32_t)((uint64_t)tiles * b / gridDim.x);
+  const uint32_t last = (uint32_t)((uint64_t)tiles * (b + 1) / gridDim.x);
   double sum = 0.0;
-  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const OptTensor& T = tensors[tile_tensor[tile]];
+  while (tile < last) {  // one tensor's share
+    const OptTensor T = tensors[tile_tensor[tile]];
     const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
-    const uint64_t end = min(base + kOptTile, T.n);
-    const G* grad = reinterpret_cast<const G*>(bucket + T.grad);
-    for (uint64_t i = base + threadIdx.x; i < end; i += kOptBlock) {
-      const double g = widen(grad[i]);
-      sum += g * g;
+    const uint64_t end = min((uint64_t)(last - T.tile0) * kOptTile, T.n);
+    gptr grad = global((const void*)(bucket + T.grad)) + base * sizeof(G);
+    uint64_t left = end - base;
+    for (; left >= kTurn; left -= kTurn, grad += kTurn * sizeof(G)) {
+      typename Words<G>::type x[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) x[u] = ldv<typename Words<G>::type>(grad, (u * kOptBlock + threadIdx.x) * 16);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) add_squares<G>(x[u][j], sum);
+      }
     }
+    for (uint32_t i = threadIdx.x; i < left; i += kOptBlock) {
+      const double g = At<G>::load(grad, i);
+      sum = fma(g, g, sum);
+    }
+    tile = (uint32_t)min((uint64_t)last, T.tile0 + (T.n + kOptTile - 1) / kOptTile);
   }
   sum = block_sum(sum, lds);
-  if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+  if (threadIdx.x == 0) partials[b] = sum;
 }
 
 __device__ __forceinline__ void finish_norm(double sum, const OptNorm& a, hydra_adamw_ctrl_t* c) {
@@ -221,40 +543,73 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_finish(const double* partial
 }
 
 // ---- 8-bit moments from and to values ---------------------------------------------------------------
+// A wave per block of 256, 4 elements per lane.
 template <typename E>
 __global__ __launch_bounds__(kOptBlock) void k_encode(uint8_t* m8, float* ms, uint8_t* v8,
                                                       float* vs, const E* m, const E* v, size_t n) {
-  __shared__ float lds[4];
-  const size_t i = (size_t)blockIdx.x * kMomentBlock + threadIdx.x;
-  const float x = m && i < n ? widen(m[i]) : 0.0f;
-  const float root = v && i < n ? sqrtf(fabsf(widen(v[i]))) : 0.0f;
-  const float sm = moment_scale(block_max(finite_abs(x), lds));
-  const float sv = moment_scale(block_max(finite_abs(root), lds));
-  if (i < n) {
-    if (m) m8[i] = (uint8_t)encode_m(x, moment_inv(sm), 0x8000u);
-    if (v) v8[i] = (uint8_t)encode_root(root, moment_inv(sv), 0x8000u);
+  const uint32_t lane = threadIdx.x & 63;
+  const size_t row = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const size_t at = row * kMomentBlock;
+  if (at >= n) return;  // whole waves
+  const uint32_t i = lane * 4, left = (uint32_t)min(n - at, (size_t)kMomentBlock);
+  const uint32_t count = left > i ? left - i : 0u;
+  f4 x = {0, 0, 0, 0}, root = {0, 0, 0, 0};
+  if (m) x = load_upto4<E>(global(m + at), i, count);
+  if (v) root = load_upto4<E>(global(v + at), i, count);
+  float fm = 0.0f, fr = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    root[j] = sqrtf(fabsf(root[j]));
+    fm = fmaxf(fm, finite_abs(x[j]));
+    fr = fmaxf(fr, finite_abs(root[j]));
   }
-  if (threadIdx.x == 0) {
-    if (m) ms[blockIdx.x] = sm;
-    if (v) vs[blockIdx.x] = sv;
+  const float scale = moment_scale(bitsf(wave_umax_pair(fbits(fm), fbits(fr))));
+  const float im = moment_inv(uniform(scale, 31)), iv = moment_inv(uniform(scale, 63));
+  uint32_t wm = 0, wv = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    wm |= encode_m(x[j], im, 0x8000u) << (8 * j);
+    wv |= encode_root(root[j], iv, 0x8000u) << (8 * j);
   }
+  if (m) store_bytes(global(m8 + at), i, wm, count);
+  if (v) store_bytes(global(v8 + at), i, wv, count);
+  if (m && lane == 31) ms[row] = scale;
+  if (v && lane == 63) vs[row] = scale;
 }
 
 template <typename E>
 __global__ __launch_bounds__(kOptBlock) void k_decode(E* m, E* v, const uint8_t* m8,
                                                       const float* ms, const uint8_t* v8,
                                                       const float* vs, size_t n) {
-  const size_t i = (size_t)blockIdx.x * kMomentBlock + threadIdx.x;
-  if (i >= n) return;
-  if (m) narrow(decode_m(m8[i], ms[blockIdx.x]), &m[i]);
-  if (v) narrow(decode_v(v8[i], vs[blockIdx.x]), &v[i]);
+  const uint32_t lane = threadIdx.x & 63;
+  const size_t row = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const size_t at = row * kMomentBlock;
+  if (at >= n) return;
+  const uint32_t i = lane * 4, left = (uint32_t)min(n - at, (size_t)kMomentBlock);
+  const uint32_t count = left > i ? left - i : 0u;
+  uint32_t cm = 0, cv = 0;
+  if (m) cm = load_bytes(global(m8 + at), i, count);
+  if (v) cv = load_bytes(global(v8 + at), i, count);
+  const float sm = m ? ms[row] : 0.0f, sv = v ? vs[row] : 0.0f;
+  f4 x, y;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    x[j] = decode_m((cm >> (8 * j)) & 255u, sm);
+    y[j] = decode_v((cv >> (8 * j)) & 255u, sv);
+  }
+  if (m) store_upto4<E>(global(m + at), i, x, count);
+  if (v) store_upto4<E>(global(v + at), i, y, count);
 }
 
 // ---- launch ------------------------------------------------------------------------------------------
 template <typename P, typename G, bool MASTER, bool S8>
 hipError_t adamw_t(const OptTable& t, const OptStep& st, const void* bucket, hipStream_t s) {
-  hipLaunchKernelGGL((k_adamw<P, G, MASTER, S8>), dim3(t.tiles), dim3(kOptBlock), 0, s, t.tensors,
-                     t.tile_tensor, st, reinterpret_cast<uint64_t>(bucket));
+  if constexpr (S8)
+    hipLaunchKernelGGL((k_adamw8<P, G, MASTER>), dim3(t.tiles), dim3(kOptBlock), 0, s, t.tensors,
+                       t.tile_tensor, t.tiles, st, reinterpret_cast<uint64_t>(bucket));
+  else
+    hipLaunchKernelGGL((k_adamw<P, G, MASTER>), dim3(t.tiles), dim3(kOptBlock), 0, s, t.tensors,
+                       t.tile_tensor, t.tiles, st, reinterpret_cast<uint64_t>(bucket));
   return hipGetLastError();
 }
 
@@ -302,7 +657,7 @@ hipError_t encode_t(uint8_t* m8, float* ms, uint8_t* v8, float* vs, const E* m, 
                     size_t n, hipStream_t s) {
   for (size_t at = 0; at < n; at += kPart) {
     const size_t part = std::min(n - at, kPart), row = at / kMomentBlock;
-    hipLaunchKernelGGL((k_encode<E>), dim3((unsigned)((part + kMomentBlock - 1) / kMomentBlock)),
+    hipLaunchKernelGGL((k_encode<E>), dim3((unsigned)((part + 4 * kMomentBlock - 1) / (4 * kMomentBlock))),
                        dim3(kOptBlock), 0, s, after(m8, at), after(ms, row), after(v8, at),
                        after(vs, row), after(m, at), after(v, at), part);
     const hipError_t e = hipGetLastError();
@@ -316,7 +671,7 @@ hipError_t decode_t(E* m, E* v, const uint8_t* m8, const float* ms, const uint8_
                     const float* vs, size_t n, hipStream_t s) {
   for (size_t at = 0; at < n; at += kPart) {
     const size_t part = std::min(n - at, kPart), row = at / kMomentBlock;
-    hipLaunchKernelGGL((k_decode<E>), dim3((unsigned)((part + kMomentBlock - 1) / kMomentBlock)),
+    hipLaunchKernelGGL((k_decode<E>), dim3((unsigned)((part + 4 * kMomentBlock - 1) / (4 * kMomentBlock))),
                        dim3(kOptBlock), 0, s, after(m, at), after(v, at), after(m8, at),
                        after(ms, row), after(v8, at), after(vs, row), part);
     const hipError_t e = hipGetLastError();

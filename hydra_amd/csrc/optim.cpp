@@ -132,6 +132,40 @@ bool touches(const std::vector<Range>& sorted, const Range& r) {
   return it != sorted.begin() && std::prev(it)->hi > r.lo;
 }
 
+// Elements before a tensor's first vector of four: those that leave the most bytes on their natural
+// alignment (16 bytes for four fp32, 8 for four 16-bit values).  Tensors that are views of flat
+// buffers of one layout are all aligned by the same head.  8-bit moments have none: their blocks
+// count from the first element.
+uint32_t head_of(const hydra_adamw_config_t& c, const hydra_adamw_tensor_t& t) {
+  if (!(c.flags & HYDRA_ADAMW_NORM_ONLY) && c.state_dtype == HYDRA_UINT8) return 0;
+  uint32_t best = 0;
+  size_t most = 0;
+  for (uint32_t h = 0; h < 4; h++) {
+    size_t on = 0;
+    auto add = [&](const void* p, size_t es, size_t passes) {
+      if ((reinterpret_cast<uintptr_t>(p) / es + h) % 4 == 0) on += es * passes;
+    };
+    add(t.grad, hydra::dtype_size(c.grad_dtype), 1);  // (a bucket's address: taken as aligned)
+    if (!(c.flags & HYDRA_ADAMW_NORM_ONLY)) {
+      add(t.param, hydra::dtype_size(c.param_dtype), t.master ? 1 : 2);  // only written, or both
+      if (t.master) add(t.master, 4, 2);
+      add(t.m, 4, 2);
+      add(t.v, 4, 2);
+    }
+    if (on > most) {
+      most = on;
+      best = h;
+    }
+  }
+  return (uint32_t)std::min<size_t>(best, t.n);
+}
+
+// Tiles of a tensor: at least one where there are elements.
+size_t tiles_of(size_t n, uint32_t head) {
+  if (n == 0) return 0;
+  return std::max<size_t>(1, (n - head + hydra::kOptTile - 1) / hydra::kOptTile);
+}
+
 int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_tensor_t* tensors,
            size_t count, hydra_adamw** made) {
   if (!config) return fail(HYDRA_ERR_INVALID, "null config");
@@ -141,7 +175,7 @@ int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_ten
   size_t tiles = 0;
   for (size_t i = 0; i < count; i++) {
     if (int rc = check_tensor(i, *config, tensors[i], &written, &grads)) return rc;
-    tiles += (tensors[i].n + hydra::kOptTile - 1) / hydra::kOptTile;
+    tiles += tiles_of(tensors[i].n, head_of(*config, tensors[i]));
   }
   if (tiles > kMaxTiles || count >= (size_t(1) << 31))
     return fail(HYDRA_ERR_INVALID, "too many elements for one plan: split it");
@@ -195,8 +229,9 @@ int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_ten
     const hydra_adamw_tensor_t& t = tensors[i];
     desc[i] = {static_cast<char*>(t.param), t.master, reinterpret_cast<uint64_t>(t.grad),
                static_cast<char*>(t.m), static_cast<char*>(t.v), t.m_scale, t.v_scale, t.n,
-               t.lr_scale, t.weight_decay, tile, (uint32_t)i};
-    for (size_t k = 0; k < t.n; k += hydra::kOptTile) of_tile[tile++] = (uint32_t)i;
+               t.lr_scale, t.weight_decay, tile, (uint32_t)i, head_of(*config, t), 0};
+    desc[i].tiles = (uint32_t)tiles_of(t.n, desc[i].head);
+    for (uint32_t k = 0; k < desc[i].tiles; k++) of_tile[tile++] = (uint32_t)i;
   }
   hipStream_t s = nullptr;
   hipError_t e = hydra::cached_stream(device, &s);

@@ -11,11 +11,13 @@ namespace hydra {
 
 constexpr int kOptBlock = 256;      // 4 waves of 64 lanes
 constexpr int kMomentBlock = 256;   // elements that share one scale of an 8-bit moment
-constexpr size_t kOptTile = 4096;   // elements of one tensor that a workgroup takes
+constexpr size_t kOptTile = 1024;   // elements of one tensor that a workgroup takes
 constexpr int kNormBlocks = 1024;   // workgroups (and partial sums) of the norm, at most
 
 // One tensor of a plan, in device memory.  `grad` counts from the bucket that a call gives (null:
-// an address).  Its tiles are [tile0, the next tensor's tile0).
+// an address).  Its tile k is number tile0 + k and holds the elements [head + k * kOptTile,
+// head + (k + 1) * kOptTile), the first one those before them too: `head` (0 to 3) puts the vectors
+// of as many of its buffers as possible on their natural alignment.
 struct OptTensor {
   char* param;
   float* master;
@@ -27,6 +29,7 @@ struct OptTensor {
   uint64_t n;
   float lr_scale, weight_decay;
   uint32_t tile0, index;
+  uint32_t head, tiles;
 };
 
 // What a plan's launches need, on the host.

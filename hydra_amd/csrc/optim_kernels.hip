@@ -65,7 +65,6 @@ __device__ __forceinline__ gptr global(const void* p) { return (gptr)(uint64_t)p
 // Four consecutive elements of any alignment (that of the element): tensors are views into buckets.
 // gfx950 runs in unaligned access mode, so these stay single 16-, 8- and 4-byte accesses.
 typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t w4h __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t w1 __attribute__((aligned(1)));
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -215,71 +214,63 @@ __device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, 
   p = p * k.decay - (m / denom) * k.size;
 }
 
-// fp32 moments: one tile of one tensor per workgroup, 4 elements per lane and turn, the loads of U
-// turns in flight at once.
-#ifndef OPT_U
-#define OPT_U 1
-#endif
+// fp32 moments: a workgroup takes one tile, 4 elements per lane.
 template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
                                                      const uint32_t* tile_tensor, uint32_t tiles,
                                                      OptStep st, uint64_t bucket) {
-  constexpr int U = OPT_U;
-  constexpr uint32_t kTurn = kOptBlock * 4 * U;
   const uint32_t tile = xcd_tile(blockIdx.x, tiles);
   const OptTensor T = tensors[tile_tensor[tile]];
   Scalars k;
   if (!load_scalars(st, T, &k)) return;
-  const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
+  const uint64_t base = T.head + (uint64_t)(tile - T.tile0) * kOptTile;
   const uint32_t left = (uint32_t)min(T.n - base, (uint64_t)kOptTile);
   const gptr grad = global((const void*)(bucket + T.grad)) + base * sizeof(G);
   const gptr param = global(T.param) + base * sizeof(P), master = global(T.master) + base * 4;
   const gptr mm = global(T.m) + base * 4, vv = global(T.v) + base * 4;
-  uint32_t i0 = 0;
-  for (; i0 + kTurn <= left; i0 += kTurn) {
-    typename At<P>::raw p[U];
-    typename At<G>::raw g[U];
-    w4 w[U], m[U], v[U];
+  const uint32_t i = threadIdx.x * 4;
+  if (i + 4 <= left) {
+    typename At<P>::raw p;
+    w4 w;
+    if (MASTER) w = At<float>::load4(master, i);
+    else p = At<P>::load4(param, i);
+    const f4 y = At<G>::wide(At<G>::load4(grad, i));
+    f4 a = At<float>::wide(At<float>::load4(mm, i)), b = At<float>::wide(At<float>::load4(vv, i));
+    f4 x = MASTER ? At<float>::wide(w) : At<P>::wide(p);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t i = i0 + (u * kOptBlock + threadIdx.x) * 4;
-      if (MASTER) w[u] = At<float>::load4(master, i);
-      else p[u] = At<P>::load4(param, i);
-      g[u] = At<G>::load4(grad, i);
-      m[u] = At<float>::load4(mm, i);
-      v[u] = At<float>::load4(vv, i);
+    for (int j = 0; j < 4; j++) {
+      float xj = x[j], aj = a[j], bj = b[j];
+      adamw(xj, y[j], aj, bj, k);
+      x[j] = xj, a[j] = aj, b[j] = bj;
     }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint32_t i = i0 + (u * kOptBlock + threadIdx.x) * 4;
-      f4 x = MASTER ? At<float>::wide(w[u]) : At<P>::wide(p[u]);
-      f4 a = At<float>::wide(m[u]), b = At<float>::wide(v[u]);
-      const f4 y = At<G>::wide(g[u]);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        float xj = x[j], aj = a[j], bj = b[j];
-        adamw(xj, y[j], aj, bj, k);
-        x[j] = xj, a[j] = aj, b[j] = bj;
-      }
-      if (MASTER) At<float>::store4(master, i, x);
-      At<P>::store4(param, i, x);
-      At<float>::store4(mm, i, a);
-      At<float>::store4(vv, i, b);
-    }
+    if (MASTER) At<float>::store4(master, i, x);
+    At<P>::store4(param, i, x);
+    At<float>::store4(mm, i, a);
+    At<float>::store4(vv, i, b);
   }
-  for (uint32_t i = i0 + threadIdx.x; i < left; i += kOptBlock) {  // the tensor's last elements
-    float p = MASTER ? At<float>::load(master, i) : At<P>::load(param, i);
-    float m = At<float>::load(mm, i), v = At<float>::load(vv, i);
-    adamw(p, At<G>::load(grad, i), m, v, k);
-    At<float>::store(mm, i, m);
-    At<float>::store(vv, i, v);
-    if (MASTER) At<float>::store(master, i, p);
-    At<P>::store(param, i, p);
+  // the tensor's ragged ends, one element per lane: up to 3 before the first tile's vectors (wave 0)
+  // and up to 3 after the last one's (wave 1)
+  const uint32_t before = tile == T.tile0 ? T.head : 0u, after = left & 3;
+  if (before | after) {
+    const uint32_t t = threadIdx.x;
+    int64_t e;
+    if (t < before) e = (int64_t)t - before;
+    else if (t >= 64 && t - 64 < after) e = left - after + (t - 64);
+    else return;
+    const gptr m1 = mm + e * 4, v1 = vv + e * 4, p1 = param + e * (int64_t)sizeof(P), w1 = master + e * 4;
+    float p = MASTER ? At<float>::load(w1, 0) : At<P>::load(p1, 0);
+    float m = At<float>::load(m1, 0), v = At<float>::load(v1, 0);
+    adamw(p, At<G>::load(grad + e * (int64_t)sizeof(G), 0), m, v, k);
+    At<float>::store(m1, 0, m);
+    At<float>::store(v1, 0, v);
+    if (MASTER) At<float>::store(w1, 0, p);
+    At<P>::store(p1, 0, p);
   }
 }
 
-// 8-bit moments: a wave takes one block of 256 elements per turn, 4 per lane, so a block's scales
-// are wave-uniform.
+// 8-bit moments: a workgroup takes one tile, a wave one block of 256 elements of it, 4 per lane, so a
+// block's scales are wave-uniform.
+static_assert(kOptTile == kOptBlock * 4 && kOptTile == kOptBlock / 64 * kMomentBlock, "one turn");
 __device__ __forceinline__ uint32_t wave_umax_pair(uint32_t a, uint32_t b) {
   // lanes 0-31: a over the wave's halves, lanes 32-63: b; then within 32 lanes, into lanes 31, 63
   const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
@@ -431,22 +422,21 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
   const bool fast = k.eps >= 0x1p-40f && k.eps <= 0x1p60f;
   const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
   const uint32_t left = (uint32_t)min(T.n - base, (uint64_t)kOptTile);
-  const uint32_t rlane = lane * 4 * 0x9E3779B1u;
-  for (uint32_t i0 = wave * kMomentBlock; i0 < left; i0 += kOptBlock / 64 * kMomentBlock) {
-    const uint64_t at = base + i0;  // the wave's block
-    const uint32_t count = left - i0 > lane * 4 ? left - i0 - lane * 4 : 0u;
-    const uint32_t rnd = (uint32_t)at * 0x9E3779B1u + rlane;
-    const uint32_t rkey = k.key ^ ((uint32_t)(at >> 32) * 0x85EBCA6Bu);
-    const gptr master = global(T.master) + at * 4, param = global(T.param) + at * sizeof(P);
-    const gptr grad = global((const void*)(bucket + T.grad)) + at * sizeof(G);
-    const gptr m8 = global(T.m) + at, v8 = global(T.v) + at;
-    const gptr ms = global(T.m_scale) + at / kMomentBlock * 4;
-    const gptr vs = global(T.v_scale) + at / kMomentBlock * 4;
-    if (fast)
-      block8<P, G, MASTER, true>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
-    else
-      block8<P, G, MASTER, false>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
-  }
+  const uint32_t i0 = wave * kMomentBlock;
+  if (i0 >= left) return;  // whole waves
+  const uint64_t at = base + i0;  // the wave's block
+  const uint32_t count = left - i0 > lane * 4 ? left - i0 - lane * 4 : 0u;
+  const uint32_t rnd = ((uint32_t)at + lane * 4) * 0x9E3779B1u;
+  const uint32_t rkey = k.key ^ ((uint32_t)(at >> 32) * 0x85EBCA6Bu);
+  const gptr master = global(T.master) + at * 4, param = global(T.param) + at * sizeof(P);
+  const gptr grad = global((const void*)(bucket + T.grad)) + at * sizeof(G);
+  const gptr m8 = global(T.m) + at, v8 = global(T.v) + at;
+  const gptr ms = global(T.m_scale) + at / kMomentBlock * 4;
+  const gptr vs = global(T.v_scale) + at / kMomentBlock * 4;
+  if (fast)
+    block8<P, G, MASTER, true>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
+  else
+    block8<P, G, MASTER, false>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
 }
 
 // ---- the norm --------------------------------------------------------------------------------------
@@ -462,8 +452,6 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
 #ifndef NORM_U
 #define NORM_U 4
 #endif
-template <typename G> struct Words { typedef w4h type; };  // 16 bytes of gradients
-template <> struct Words<float> { typedef w4 type; };
 // the squares of a dword's gradients
 template <typename G>
 __device__ __forceinline__ void add_squares(uint32_t w, double& sum) {
@@ -484,33 +472,55 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* ten
                                                             uint32_t tiles, uint64_t bucket,
                                                             double* partials) {
   constexpr int N = 16 / sizeof(G), U = NORM_U;  // elements of a 16-byte load, loads in flight
-  constexpr uint32_t kTurn = kOptBlock * N * U;
   __shared__ double lds[4];
   const uint32_t b = xcd_tile(blockIdx.x, gridDim.x);
   uint32_t tile = (uint32_t)((uint64_t)tiles * b / gridDim.x);
   const uint32_t last = (uint32_t)((uint64_t)tiles * (b + 1) / gridDim.x);
   double sum = 0.0;
-  while (tile < last) {  // one tensor's share
+  while (tile < last) {  // one tensor's share: [from, to)
     const OptTensor T = tensors[tile_tensor[tile]];
-    const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
-    const uint64_t end = min((uint64_t)(last - T.tile0) * kOptTile, T.n);
-    gptr grad = global((const void*)(bucket + T.grad)) + base * sizeof(G);
-    uint64_t left = end - base;
-    for (; left >= kTurn; left -= kTurn, grad += kTurn * sizeof(G)) {
-      typename Words<G>::type x[U];
+    const uint32_t first = tile - T.tile0, end = min(last - T.tile0, T.tiles);
+    const uint64_t from = first ? T.head + first * (uint64_t)kOptTile : 0;
+    const uint64_t to = min(T.head + end * (uint64_t)kOptTile, T.n);
+    const uint64_t addr = bucket + T.grad + from * sizeof(G), n = to - from;
+    const uint32_t head = (uint32_t)min((uint64_t)((16 - (addr & 15)) & 15) / sizeof(G), n);
+    const uint64_t vecs = (n - head) / N;
+    const uint32_t tail = (uint32_t)(n - head - vecs * N);
+    const gptr ends = global((const void*)addr);
+    if (threadIdx.x < head) {
+      const double g = At<G>::load(ends, threadIdx.x);
+      sum = fma(g, g, sum);
+    } else if (threadIdx.x >= 64 && threadIdx.x - 64 < tail) {
+      const double g = At<G>::load(ends + (head + vecs * N) * sizeof(G), threadIdx.x - 64);
+      sum = fma(g, g, sum);
+    }
+    gptr at = ends + head * sizeof(G);
+    uint64_t left = vecs;
+    for (; left >= kOptBlock * U; left -= kOptBlock * U, at += kOptBlock * U * 16) {
+      w4 x[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) x[u] = ldv<typename Words<G>::type>(grad, (u * kOptBlock + threadIdx.x) * 16);
+      for (int u = 0; u < U; u++) x[u] = ldv<w4>(at, (u * kOptBlock + threadIdx.x) * 16);
 #pragma unroll
       for (int u = 0; u < U; u++) {
 #pragma unroll
         for (int j = 0; j < 4; j++) add_squares<G>(x[u][j], sum);
       }
     }
-    for (uint32_t i = threadIdx.x; i < left; i += kOptBlock) {
-      const double g = At<G>::load(grad, i);
-      sum = fma(g, g, sum);
+    if (left) {  // the last turn: vectors that are not there count as zeros
+      w4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const uint32_t v = u * kOptBlock + threadIdx.x;
+        x[u] = w4{0, 0, 0, 0};
+        if (v < left) x[u] = ldv<w4>(at, v * 16);
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) add_squares<G>(x[u][j], sum);
+      }
     }
-    tile = (uint32_t)min((uint64_t)last, T.tile0 + (T.n + kOptTile - 1) / kOptTile);
+    tile = T.tile0 + end;
   }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) partials[b] = sum;

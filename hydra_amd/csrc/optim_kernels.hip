@@ -65,7 +65,9 @@ __device__ __forceinline__ gptr global(const void* p) { return (gptr)(uint64_t)p
 // Four consecutive elements of any alignment (that of the element): tensors are views into buckets.
 // gfx950 runs in unaligned access mode, so these stay single 16-, 8- and 4-byte accesses.
 typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t w4h __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t w2b __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t w1 __attribute__((aligned(1)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 // Nontemporal both ways: a step's state is larger than the caches.  64 Mi fp32: 344 us, against 368
@@ -98,6 +100,10 @@ template <> struct At<float> {
   __device__ __forceinline__ static void store4(gptr p, uint32_t i, f4 x) {
     stv<w4>(p, i * 4, w4{fbits(x[0]), fbits(x[1]), fbits(x[2]), fbits(x[3])});
   }
+  __device__ __forceinline__ static void store8(gptr p, uint32_t i, f4 x, f4 y) {
+    store4(p, i, x);
+    store4(p, i + 4, y);
+  }
 };
 template <> struct At<bf16_t> {
   __device__ __forceinline__ static float load(gptr p, uint32_t i) { return bf2f(*(const GLOBAL uint16_t*)(p + i * 2)); }
@@ -109,10 +115,15 @@ template <> struct At<bf16_t> {
   __device__ __forceinline__ static f4 wide(raw r) {
     return f4{bitsf(r[0] << 16), bitsf(r[0] & 0xffff0000u), bitsf(r[1] << 16), bitsf(r[1] & 0xffff0000u)};
   }
-  __device__ __forceinline__ static void store4(gptr p, uint32_t i, f4 x) {
+  __device__ __forceinline__ static uint32_t pair(float x, float y) {
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 lo{(__bf16)x[0], (__bf16)x[1]}, hi{(__bf16)x[2], (__bf16)x[3]};
-    stv<w2>(p, i * 2, w2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)});
+    return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+  }
+  __device__ __forceinline__ static void store4(gptr p, uint32_t i, f4 x) {
+    stv<w2>(p, i * 2, w2{pair(x[0], x[1]), pair(x[2], x[3])});
+  }
+  __device__ __forceinline__ static void store8(gptr p, uint32_t i, f4 x, f4 y) {
+    stv<w4h>(p, i * 2, w4h{pair(x[0], x[1]), pair(x[2], x[3]), pair(y[0], y[1]), pair(y[2], y[3])});
   }
 };
 template <> struct At<f16_t> {
@@ -271,10 +282,8 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
 // 8-bit moments: a workgroup takes one tile, a wave one block of 256 elements of it, 4 per lane, so a
 // block's scales are wave-uniform.
 static_assert(kOptTile == kOptBlock * 4 && kOptTile == kOptBlock / 64 * kMomentBlock, "one turn");
-__device__ __forceinline__ uint32_t wave_umax_pair(uint32_t a, uint32_t b) {
-  // lanes 0-31: a over the wave's halves, lanes 32-63: b; then within 32 lanes, into lanes 31, 63
-  const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-  uint32_t x = max((uint32_t)s[0], (uint32_t)s[1]);
+// lanes 31 and 63: the largest of their half of the wave
+__device__ __forceinline__ uint32_t half_wave_umax(uint32_t x) {
 #define HYDRA_DPP_MAX(ctrl) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true))
   HYDRA_DPP_MAX(0x111);  // row_shr:1
   HYDRA_DPP_MAX(0x112);
@@ -283,6 +292,12 @@ __device__ __forceinline__ uint32_t wave_umax_pair(uint32_t a, uint32_t b) {
   HYDRA_DPP_MAX(0x142);  // row_bcast:15
 #undef HYDRA_DPP_MAX
   return x;
+}
+// lane 31: the wave's largest a, lane 63: its largest b (the halves of a meet in lanes 0-31, those of
+// b in the others)
+__device__ __forceinline__ uint32_t wave_umax_pair(uint32_t a, uint32_t b) {
+  const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  return half_wave_umax(max((uint32_t)s[0], (uint32_t)s[1]));
 }
 // c + (low / high half of r) * 16 or * 8: the 16 random bits at the top of what the cut drops
 __device__ __forceinline__ uint32_t add_low16(uint32_t c, uint32_t r) {
@@ -295,6 +310,37 @@ __device__ __forceinline__ uint32_t add_high16(uint32_t c, uint32_t r) {
   asm("v_mad_u32_u16 %0, %1, 8, %2 op_sel:[1,0,0,0]" : "=v"(d) : "v"(r), "v"(c));
   return d;
 }
+// What a block's largest magnitude (its bits) has to be for the encoders below: 2^-112 / scale is
+// normal, and every value is finite.  sqrt v also not below 2^-44: the hardware's square root takes
+// what is below 2^-126 for 0, and what that hides then lies under the smallest byte.
+__device__ __forceinline__ bool plain_m(uint32_t top) { return top < fbits(0x1p14f); }
+__device__ __forceinline__ bool plain_root(uint32_t top) {
+  return top - fbits(0x1p-44f) < fbits(0x1p14f) - fbits(0x1p-44f);
+}
+// 2^-112 / scale to within 1 ulp (0 for an empty block)
+__device__ __forceinline__ float plain_inv(float scale) {
+  return scale > 0.0f ? __builtin_amdgcn_rcpf(scale) * 0x1p-112f : 0.0f;
+}
+// The bytes of four values of plain blocks; add(c, j) rounds c by the random bits of element j.
+template <typename F>
+__device__ __forceinline__ uint32_t encode4_m(f4 m, float inv, F add) {
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) c[j] = min(add(fbits(fabsf(m[j]) * inv), j) >> 20, 127u);
+  const uint32_t w = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+  // the four signs, but not of zeros
+  const uint32_t signs = __builtin_amdgcn_perm(fbits(m[3]), fbits(m[2]), 0x07030c0cu) |
+                         __builtin_amdgcn_perm(fbits(m[1]), fbits(m[0]), 0x0c0c0703u);
+  return w | (signs & (w + 0x7f7f7f7fu) & 0x80808080u);
+}
+template <typename F>
+__device__ __forceinline__ uint32_t encode4_root(f4 root, f4 v, float inv, F add) {
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++)  // 0 for v = 0 alone
+    c[j] = min(min(max(add(fbits(root[j] * inv), j) >> 19, 1u), 254u), fbits(v[j]));
+  return c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+}
 __device__ __forceinline__ uint32_t zero_bytes(uint32_t x) {  // not 0 where x has a byte of 0
   return (x - 0x01010101u) & ~x & 0x80808080u;
 }
@@ -302,13 +348,11 @@ __device__ __forceinline__ float uniform(float x, int lane) {
   return bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(x), lane));
 }
 
-// A block's four elements per lane: decode, step, encode.  FAST needs eps in [2^-40, 2^60].  Its
-// shortcuts: no byte that stands for something not finite and both old scales below 2^15 (so
-// 2^112 * scale is finite: one product per value); sqrt and the reciprocal by the hardware's own
-// instructions (1 ulp; they flush below 2^-126, where eps hides it); and new magnitudes whose
-// largest lie in [2^-44, 2^14) (sqrt v) and below 2^14 (m), so that what sqrt flushed is below a
-// byte's smallest step and 2^-112 / scale is normal.  A block that is outside takes the general
-// code for that half.
+// A block's four elements per lane: decode, step, encode.  FAST needs eps in [2^-40, 2^60]: the
+// square root and the reciprocal are the hardware's own then (1 ulp; what they flush eps hides).
+// Decoding is short where no byte stands for something not finite and both old scales are below
+// 2^15 (2^112 * scale is finite: one product per value), encoding where the block is plain (above).
+// A block that is not takes the general code for that half.
 template <typename P, typename G, bool MASTER, bool FAST>
 __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr m8, gptr v8,
                                        gptr ms, gptr vs, uint32_t count, uint32_t lane,
@@ -358,32 +402,19 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
   const uint32_t top = wave_umax_pair(am, ar);
   const uint32_t tm = (uint32_t)__builtin_amdgcn_readlane((int)top, 31);
   const uint32_t tr = (uint32_t)__builtin_amdgcn_readlane((int)top, 63);
-  float scale, s_m, s_v;
-  uint32_t em[4], ev[4], r[4];
+  float scale;
+  uint32_t r[4], wm, wv;
 #pragma unroll
   for (int j = 0; j < 4; j++) r[j] = 0x80008000u;
   if (k.stochastic) {
 #pragma unroll
     for (int j = 0; j < 4; j++) r[j] = fmix32((rnd + j * 0x9E3779B1u) ^ rkey);
   }
-  uint32_t wm, wv;
-  if (!odd && tm < fbits(0x1p14f) && tr - fbits(0x1p-44f) < fbits(0x1p14f) - fbits(0x1p-44f)) {
-    const bool none = top < fbits(kTiny);
-    scale = none ? 0.0f : bitsf(top) * kTop;
-    const float inv = none ? 0.0f : __builtin_amdgcn_rcpf(scale) * 0x1p-112f;
-    const float im = uniform(inv, 31), iv = uniform(inv, 63);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      em[j] = min(add_low16(fbits(fabsf(m[j]) * im), r[j]) >> 20, 127u);
-      const uint32_t c = add_high16(fbits(root[j] * iv), r[j]) >> 19;
-      ev[j] = min(min(max(c, 1u), 254u), fbits(v[j]));  // 0 for v = 0 alone
-    }
-    wm = em[0] | em[1] << 8 | em[2] << 16 | em[3] << 24;
-    wv = ev[0] | ev[1] << 8 | ev[2] << 16 | ev[3] << 24;
-    // the signs, but not of zeros
-    const uint32_t hi = __builtin_amdgcn_perm(fbits(m[3]), fbits(m[2]), 0x07030c0cu) |
-                        __builtin_amdgcn_perm(fbits(m[1]), fbits(m[0]), 0x0c0c0703u);
-    wm |= hi & (wm + 0x7f7f7f7fu) & 0x80808080u;
+  if (!odd && plain_m(tm) && plain_root(tr)) {
+    scale = moment_scale(bitsf(top));
+    const float inv = plain_inv(scale);
+    wm = encode4_m(m, uniform(inv, 31), [&](uint32_t c, int j) { return add_low16(c, r[j]); });
+    wv = encode4_root(root, v, uniform(inv, 63), [&](uint32_t c, int j) { return add_high16(c, r[j]); });
   } else {
     float fm = 0.0f, fr = 0.0f;
 #pragma unroll
@@ -393,8 +424,7 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
       fr = fmaxf(fr, finite_abs(root[j]));
     }
     scale = moment_scale(bitsf(wave_umax_pair(fbits(fm), fbits(fr))));
-    s_m = uniform(scale, 31), s_v = uniform(scale, 63);
-    const float im = moment_inv(s_m), iv = moment_inv(s_v);
+    const float im = moment_inv(uniform(scale, 31)), iv = moment_inv(uniform(scale, 63));
     wm = wv = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -553,62 +583,132 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_finish(const double* partial
 }
 
 // ---- 8-bit moments from and to values ---------------------------------------------------------------
-// A wave per block of 256, 4 elements per lane.
+// Two blocks of 256 per wave.
+constexpr size_t kConvTile = kOptBlock / 64 * 2 * kMomentBlock;  // elements of a workgroup
+
+// a wave's first element, and how many (up to 512) it has
+__device__ __forceinline__ uint32_t wave_part(size_t n, size_t* at) {
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  *at = (size_t)xcd_tile(blockIdx.x, gridDim.x) * kConvTile + wave * (2 * kMomentBlock);
+  return *at < n ? (uint32_t)min(n - *at, (size_t)(2 * kMomentBlock)) : 0u;
+}
+__device__ __forceinline__ uint32_t rest(uint32_t left, uint32_t i) { return left > i ? left - i : 0u; }
+
+// encode: 4 elements per lane of each block, all loads first (8 consecutive ones per lane leave every
+// fp32 load half of the lines it touches)
 template <typename E>
 __global__ __launch_bounds__(kOptBlock) void k_encode(uint8_t* m8, float* ms, uint8_t* v8,
                                                       float* vs, const E* m, const E* v, size_t n) {
-  const uint32_t lane = threadIdx.x & 63;
-  const size_t row = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const size_t at = row * kMomentBlock;
-  if (at >= n) return;  // whole waves
-  const uint32_t i = lane * 4, left = (uint32_t)min(n - at, (size_t)kMomentBlock);
-  const uint32_t count = left > i ? left - i : 0u;
-  f4 x = {0, 0, 0, 0}, root = {0, 0, 0, 0};
-  if (m) x = load_upto4<E>(global(m + at), i, count);
-  if (v) root = load_upto4<E>(global(v + at), i, count);
-  float fm = 0.0f, fr = 0.0f;
+  size_t at;
+  const uint32_t left = wave_part(n, &at), lane = threadIdx.x & 63;
+  if (!left) return;
+  f4 x[2], y[2];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    root[j] = sqrtf(fabsf(root[j]));
-    fm = fmaxf(fm, finite_abs(x[j]));
-    fr = fmaxf(fr, finite_abs(root[j]));
+  for (int h = 0; h < 2; h++) {
+    const uint32_t i = h * kMomentBlock + lane * 4;
+    x[h] = y[h] = f4{0, 0, 0, 0};
+    if (m) x[h] = load_upto4<E>(global(m + at), i, rest(left, i));
+    if (v) y[h] = load_upto4<E>(global(v + at), i, rest(left, i));
   }
-  const float scale = moment_scale(bitsf(wave_umax_pair(fbits(fm), fbits(fr))));
-  const float im = moment_inv(uniform(scale, 31)), iv = moment_inv(uniform(scale, 63));
-  uint32_t wm = 0, wv = 0;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    wm |= encode_m(x[j], im, 0x8000u) << (8 * j);
-    wv |= encode_root(root[j], iv, 0x8000u) << (8 * j);
+  for (int h = 0; h < 2; h++) {
+    if (h * kMomentBlock >= left) break;
+    const uint32_t i = h * kMomentBlock + lane * 4, count = rest(left, i);
+    f4 root;
+    uint32_t am = 0, ar = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      y[h][j] = fabsf(y[h][j]);
+      root[j] = __builtin_amdgcn_sqrtf(y[h][j]);
+      am = max(am, fbits(fabsf(x[h][j])));
+      ar = max(ar, fbits(root[j]));
+    }
+    const uint32_t top = wave_umax_pair(am, ar);
+    const uint32_t tm = (uint32_t)__builtin_amdgcn_readlane((int)top, 31);
+    const uint32_t tr = (uint32_t)__builtin_amdgcn_readlane((int)top, 63);
+    // each moment by itself: its bytes do not depend on the other one's being given
+    const bool pm = plain_m(tm), pv = plain_root(tr);
+    float scale = moment_scale(bitsf(top));
+    if (!pm || !pv) {
+      float fm = 0.0f, fr = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (!pv) root[j] = sqrtf(y[h][j]);
+        fm = fmaxf(fm, finite_abs(x[h][j]));
+        fr = fmaxf(fr, finite_abs(root[j]));
+      }
+      scale = moment_scale(bitsf(wave_umax_pair(fbits(fm), fbits(fr))));
+    }
+    const float inv = plain_inv(scale);
+    uint32_t wm = 0, wv = 0;
+    if (pm) {
+      wm = encode4_m(x[h], uniform(inv, 31), [](uint32_t c, int) { return c + (0x8000u << 4); });
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        wm |= encode_m(x[h][j], moment_inv(uniform(scale, 31)), 0x8000u) << (8 * j);
+    }
+    if (pv) {
+      wv = encode4_root(root, y[h], uniform(inv, 63), [](uint32_t c, int) { return c + (0x8000u << 3); });
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        wv |= encode_root(root[j], moment_inv(uniform(scale, 63)), 0x8000u) << (8 * j);
+    }
+    if (m) store_bytes(global(m8 + at), i, wm, count);
+    if (v) store_bytes(global(v8 + at), i, wv, count);
+    if (m && lane == 31) ms[at / kMomentBlock + h] = scale;
+    if (v && lane == 63) vs[at / kMomentBlock + h] = scale;
   }
-  if (m) store_bytes(global(m8 + at), i, wm, count);
-  if (v) store_bytes(global(v8 + at), i, wv, count);
-  if (m && lane == 31) ms[row] = scale;
-  if (v && lane == 63) vs[row] = scale;
+}
+
+// decode: 8 consecutive elements per lane
+struct Part {
+  uint32_t i, count, lo, hi;  // the lane's first element; how many it has, in all and by fours
+};
+struct Coded {
+  w2b w;
+  float scale;
+};
+__device__ __forceinline__ Coded load_codes(gptr codes, gptr scales, const Part& p) {
+  Coded c;
+  c.scale = At<float>::load(scales, (threadIdx.x >> 5) & 1);
+  if (p.count >= 8) c.w = ldv<w2b>(codes, p.i);
+  else c.w = w2b{load_bytes(codes, p.i, p.lo), load_bytes(codes, p.i + 4, p.hi)};
+  return c;
+}
+template <typename E, bool ROOT>
+__device__ __forceinline__ void decode_part(gptr values, const Coded& c, const Part& p) {
+  f4 x[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t b = (c.w[h] >> (8 * j)) & 255u;
+      x[h][j] = ROOT ? decode_v(b, c.scale) : decode_m(b, c.scale);
+    }
+  if (p.count >= 8) {
+    At<E>::store8(values, p.i, x[0], x[1]);
+  } else {
+    store_upto4<E>(values, p.i, x[0], p.lo);
+    store_upto4<E>(values, p.i + 4, x[1], p.hi);
+  }
 }
 
 template <typename E>
 __global__ __launch_bounds__(kOptBlock) void k_decode(E* m, E* v, const uint8_t* m8,
                                                       const float* ms, const uint8_t* v8,
                                                       const float* vs, size_t n) {
-  const uint32_t lane = threadIdx.x & 63;
-  const size_t row = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const size_t at = row * kMomentBlock;
-  if (at >= n) return;
-  const uint32_t i = lane * 4, left = (uint32_t)min(n - at, (size_t)kMomentBlock);
-  const uint32_t count = left > i ? left - i : 0u;
-  uint32_t cm = 0, cv = 0;
-  if (m) cm = load_bytes(global(m8 + at), i, count);
-  if (v) cv = load_bytes(global(v8 + at), i, count);
-  const float sm = m ? ms[row] : 0.0f, sv = v ? vs[row] : 0.0f;
-  f4 x, y;
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    x[j] = decode_m((cm >> (8 * j)) & 255u, sm);
-    y[j] = decode_v((cv >> (8 * j)) & 255u, sv);
-  }
-  if (m) store_upto4<E>(global(m + at), i, x, count);
-  if (v) store_upto4<E>(global(v + at), i, y, count);
+  size_t at;
+  const uint32_t left = wave_part(n, &at), i = (threadIdx.x & 63) * 8;
+  if (i >= left) return;
+  const Part p{i, left - i, left - i, rest(left, i + 4)};
+  const size_t row = at / kMomentBlock;
+  Coded a, b;
+  if (m) a = load_codes(global(m8 + at), global(ms + row), p);
+  if (v) b = load_codes(global(v8 + at), global(vs + row), p);
+  if (m) decode_part<E, false>(global(m + at), a, p);
+  if (v) decode_part<E, true>(global(v + at), b, p);
 }
 
 // ---- launch ------------------------------------------------------------------------------------------
@@ -667,7 +767,7 @@ hipError_t encode_t(uint8_t* m8, float* ms, uint8_t* v8, float* vs, const E* m, 
                     size_t n, hipStream_t s) {
   for (size_t at = 0; at < n; at += kPart) {
     const size_t part = std::min(n - at, kPart), row = at / kMomentBlock;
-    hipLaunchKernelGGL((k_encode<E>), dim3((unsigned)((part + 4 * kMomentBlock - 1) / (4 * kMomentBlock))),
+    hipLaunchKernelGGL((k_encode<E>), dim3((unsigned)((part + kConvTile - 1) / kConvTile)),
                        dim3(kOptBlock), 0, s, after(m8, at), after(ms, row), after(v8, at),
                        after(vs, row), after(m, at), after(v, at), part);
     const hipError_t e = hipGetLastError();
@@ -681,7 +781,7 @@ hipError_t decode_t(E* m, E* v, const uint8_t* m8, const float* ms, const uint8_
                     const float* vs, size_t n, hipStream_t s) {
   for (size_t at = 0; at < n; at += kPart) {
     const size_t part = std::min(n - at, kPart), row = at / kMomentBlock;
-    hipLaunchKernelGGL((k_decode<E>), dim3((unsigned)((part + 4 * kMomentBlock - 1) / (4 * kMomentBlock))),
+    hipLaunchKernelGGL((k_decode<E>), dim3((unsigned)((part + kConvTile - 1) / kConvTile)),
                        dim3(kOptBlock), 0, s, after(m, at), after(v, at), after(m8, at),
                        after(ms, row), after(v8, at), after(vs, row), part);
     const hipError_t e = hipGetLastError();

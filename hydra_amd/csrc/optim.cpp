@@ -373,20 +373,21 @@ int hydra_adamw_destroy(hydra_adamw_t plan) {
 
 int hydra_adamw_workspace(hydra_adamw_t plan, size_t* bytes) {
   if (!plan || !bytes) return fail(HYDRA_ERR_INVALID, "null plan or bytes");
-  *bytes = hydra::norm_partials(plan->table.tiles) * sizeof(double);
+  *bytes = hydra::norm_workspace(plan->table.tiles);
   return ok();
 }
 
 int hydra_adamw_grad_norm(hydra_adamw_t plan, const void* bucket, double grad_scale,
                           double max_norm, hydra_adamw_ctrl_t* ctrl, void* workspace,
                           size_t workspace_bytes, hydra_stream_t stream) {
-  if (!plan || !ctrl || !workspace) return fail(HYDRA_ERR_INVALID, "null plan, ctrl or workspace");
+  if (!plan || !ctrl) return fail(HYDRA_ERR_INVALID, "null plan or ctrl");
   if (!std::isfinite((float)grad_scale))
     return fail(HYDRA_ERR_INVALID, "grad_scale must be finite in fp32");
   if (!(max_norm >= 0.0)) return fail(HYDRA_ERR_INVALID, "max_norm must be >= 0");
   if (!aligned(ctrl, 8) || !aligned(workspace, 8))
     return fail(HYDRA_ERR_INVALID, "ctrl and workspace must be 8-byte aligned");
-  if (workspace_bytes < hydra::norm_partials(plan->table.tiles) * sizeof(double))
+  const size_t need = hydra::norm_workspace(plan->table.tiles);
+  if (workspace_bytes < need || (need && !workspace))
     return fail(HYDRA_ERR_INVALID, "workspace smaller than hydra_adamw_workspace says");
   if (int rc = check_bucket(*plan, bucket)) return rc;
   hydra::DeviceScope ds(plan->device);

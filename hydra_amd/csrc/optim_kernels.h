@@ -72,7 +72,7 @@ __host__ __device__ inline double power(double beta, uint64_t t) {
 
 hipError_t launch_adamw(const hydra_adamw_config_t& cfg, const OptTable& t, const OptStep& step,
                         const void* bucket, hipStream_t s);
-uint32_t norm_partials(uint32_t tiles);
+size_t norm_workspace(uint32_t tiles);  // bytes of partial sums
 hipError_t launch_grad_norm(int grad_dtype, const OptTable& t, const OptNorm& norm,
                             const void* bucket, hydra_adamw_ctrl_t* ctrl, double* partials,
                             hipStream_t s);

@@ -175,8 +175,8 @@ __device__ __forceinline__ uint32_t load_bytes(gptr p, uint32_t i, uint32_t coun
   return w;
 }
 __device__ __forceinline__ void store_bytes(gptr p, uint32_t i, uint32_t w, uint32_t count) {
-  if (count >= 4) {
-    stv<w1>(p, i, w);
+  if (count >= 4) {  // not nontemporal: 4 bytes per lane are joined in the cache (178 -> 170 us)
+    *(GLOBAL w1*)(p + i) = w;
     return;
   }
 #pragma unroll
@@ -217,20 +217,24 @@ __device__ __forceinline__ bool load_scalars(const OptStep& st, const OptTensor&
   return true;
 }
 
-__device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, const Scalars& k) {
-  const float g = grad * k.mult;
+__device__ __forceinline__ void moments(float g, float& m, float& v, const Scalars& k) {
   m = m * k.b1 + g * k.omb1;
   v = v * k.b2 + (g * k.omb2) * g;
-  const float denom = sqrtf(v) * k.isb2 + k.eps;
-  p = p * k.decay - (m / denom) * k.size;
+}
+__device__ __forceinline__ float weight(float p, float m, float v, const Scalars& k) {
+  return p * k.decay - (m / (sqrtf(v) * k.isb2 + k.eps)) * k.size;
+}
+__device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, const Scalars& k) {
+  moments(grad * k.mult, m, v, k);
+  p = weight(p, m, v, k);
 }
 
 // fp32 moments: a workgroup takes one tile, 4 elements per lane.
 template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
-                                                     const uint32_t* tile_tensor, uint32_t tiles,
-                                                     OptStep st, uint64_t bucket) {
-  const uint32_t tile = xcd_tile(blockIdx.x, tiles);
+                                                     const uint32_t* tile_tensor, OptStep st,
+                                                     uint64_t bucket) {
+  const uint32_t tile = blockIdx.x;
   const OptTensor T = tensors[tile_tensor[tile]];
   Scalars k;
   if (!load_scalars(st, T, &k)) return;
@@ -310,17 +314,24 @@ __device__ __forceinline__ uint32_t add_high16(uint32_t c, uint32_t r) {
   asm("v_mad_u32_u16 %0, %1, 8, %2 op_sel:[1,0,0,0]" : "=v"(d) : "v"(r), "v"(c));
   return d;
 }
+// The square root of v >= 0, not denormal, rounded as sqrtf rounds it, in 8 issue slots instead of 17:
+// the reciprocal root's estimate s, then s + (v - s^2) / (2 s) (all 2^24 values of [1, 4) checked
+// against sqrtf; below 2^-98 the rest v - s^2 itself is rounded, and 1 ulp may be off).  A denormal
+// becomes something below 2^-63; what is not finite, something not finite.
+__device__ __forceinline__ float plain_sqrt(float v) {
+  const float r = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f));
+  const float s = v * r;
+  return fmaf(fmaf(-s, s, v), 0.5f * r, s);
+}
 // What a block's largest magnitude (its bits) has to be for the encoders below: 2^-112 / scale is
-// normal, and every value is finite.  sqrt v also not below 2^-44: the hardware's square root takes
-// what is below 2^-126 for 0, and what that hides then lies under the smallest byte.
+// normal, and every value is finite.  sqrt v also not below 2^-44: what plain_sqrt does not see in
+// denormals lies under the smallest byte then.
 __device__ __forceinline__ bool plain_m(uint32_t top) { return top < fbits(0x1p14f); }
 __device__ __forceinline__ bool plain_root(uint32_t top) {
   return top - fbits(0x1p-44f) < fbits(0x1p14f) - fbits(0x1p-44f);
 }
-// 2^-112 / scale to within 1 ulp (0 for an empty block)
-__device__ __forceinline__ float plain_inv(float scale) {
-  return scale > 0.0f ? __builtin_amdgcn_rcpf(scale) * 0x1p-112f : 0.0f;
-}
+// 2^-112 / scale (0 for an empty block)
+__device__ __forceinline__ float plain_inv(float scale) { return moment_inv(scale) * 0x1p-112f; }
 // The bytes of four values of plain blocks; add(c, j) rounds c by the random bits of element j.
 template <typename F>
 __device__ __forceinline__ uint32_t encode4_m(f4 m, float inv, F add) {
@@ -348,12 +359,12 @@ __device__ __forceinline__ float uniform(float x, int lane) {
   return bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(x), lane));
 }
 
-// A block's four elements per lane: decode, step, encode.  FAST needs eps in [2^-40, 2^60]: the
-// square root and the reciprocal are the hardware's own then (1 ulp; what they flush eps hides).
-// Decoding is short where no byte stands for something not finite and both old scales are below
-// 2^15 (2^112 * scale is finite: one product per value), encoding where the block is plain (above).
-// A block that is not takes the general code for that half.
-template <typename P, typename G, bool MASTER, bool FAST>
+// A block's four elements per lane: decode, step, encode.  The bytes are those of the documented
+// operations, each rounded to fp32.  Decoding is short where no byte stands for something not finite
+// and both old scales are below 2^15 (2^112 * scale is finite: one product per value).  The rest is
+// short where the block is plain (above) and eps lies in [2^-40, 2^60]: eps hides what plain_sqrt
+// does not see, and the quotient is a product with the hardware's reciprocal (2 ulp).
+template <typename P, typename G, bool MASTER>
 __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr m8, gptr v8,
                                        gptr ms, gptr vs, uint32_t count, uint32_t lane,
                                        uint32_t rnd, uint32_t rkey, const Scalars& k) {
@@ -364,8 +375,8 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
   const uint32_t cm = load_bytes(m8, i, count), cv = load_bytes(v8, i, count);
   const float ms0 = At<float>::load(ms, 0), vs0 = At<float>::load(vs, 0);
   f4 m, v, root;
-  bool odd = !FAST || !(ms0 < 0x1p15f && vs0 < 0x1p15f) ||
-             __any((zero_bytes(cm ^ 0x80808080u) | zero_bytes(~cv)) != 0);
+  const bool odd = !(ms0 < 0x1p15f && vs0 < 0x1p15f) ||
+                   __any((zero_bytes(cm ^ 0x80808080u) | zero_bytes(~cv)) != 0);
   if (odd) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -381,24 +392,17 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
       v[j] = r0 * r0;
     }
   }
+  uint32_t ar = 0;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    if (FAST) {
-      const float y = g[j] * k.mult;
-      m[j] = fmaf(y, k.omb1, m[j] * k.b1);
-      v[j] = fmaf(y * k.omb2, y, v[j] * k.b2);
-      root[j] = __builtin_amdgcn_sqrtf(v[j]);
-      const float denom = fmaf(root[j], k.isb2, k.eps);
-      p[j] = fmaf(m[j] * -k.size, __builtin_amdgcn_rcpf(denom), p[j] * k.decay);
-    } else {
-      float pj = p[j], mj = m[j], vj = v[j];
-      adamw(pj, g[j], mj, vj, k);
-      p[j] = pj, m[j] = mj, v[j] = vj;
-      root[j] = sqrtf(vj);
-    }
+    float mj = m[j], vj = v[j];
+    moments(g[j] * k.mult, mj, vj, k);
+    m[j] = mj, v[j] = vj;
+    root[j] = plain_sqrt(vj);
+    ar = max(ar, fbits(root[j]));
   }
+  // (a NaN among m, which the maximum passes over, has an infinite or a NaN v beside it, or was odd)
   const uint32_t am = fbits(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
-  const uint32_t ar = max(max(fbits(root[0]), fbits(root[1])), max(fbits(root[2]), fbits(root[3])));
   const uint32_t top = wave_umax_pair(am, ar);
   const uint32_t tm = (uint32_t)__builtin_amdgcn_readlane((int)top, 31);
   const uint32_t tr = (uint32_t)__builtin_amdgcn_readlane((int)top, 63);
@@ -410,7 +414,12 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
 #pragma unroll
     for (int j = 0; j < 4; j++) r[j] = fmix32((rnd + j * 0x9E3779B1u) ^ rkey);
   }
-  if (!odd && plain_m(tm) && plain_root(tr)) {
+  if (!odd && plain_m(tm) && plain_root(tr) && k.eps >= 0x1p-40f && k.eps <= 0x1p60f) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float denom = fmaf(root[j], k.isb2, k.eps);
+      p[j] = fmaf(m[j] * -k.size, __builtin_amdgcn_rcpf(denom), p[j] * k.decay);
+    }
     scale = moment_scale(bitsf(top));
     const float inv = plain_inv(scale);
     wm = encode4_m(m, uniform(inv, 31), [&](uint32_t c, int j) { return add_low16(c, r[j]); });
@@ -419,7 +428,8 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
     float fm = 0.0f, fr = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      if (FAST) root[j] = sqrtf(v[j]);
+      p[j] = weight(p[j], m[j], v[j], k);
+      root[j] = sqrtf(v[j]);
       fm = fmaxf(fm, finite_abs(m[j]));
       fr = fmaxf(fr, finite_abs(root[j]));
     }
@@ -449,7 +459,6 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
   if (!load_scalars(st, T, &k)) return;
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const bool fast = k.eps >= 0x1p-40f && k.eps <= 0x1p60f;
   const uint64_t base = (uint64_t)(tile - T.tile0) * kOptTile;
   const uint32_t left = (uint32_t)min(T.n - base, (uint64_t)kOptTile);
   const uint32_t i0 = wave * kMomentBlock;
@@ -463,25 +472,48 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
   const gptr m8 = global(T.m) + at, v8 = global(T.v) + at;
   const gptr ms = global(T.m_scale) + at / kMomentBlock * 4;
   const gptr vs = global(T.v_scale) + at / kMomentBlock * 4;
-  if (fast)
-    block8<P, G, MASTER, true>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
-  else
-    block8<P, G, MASTER, false>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
+  block8<P, G, MASTER>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
 }
 
 // ---- the norm --------------------------------------------------------------------------------------
 // fp64 sums: no gradient's square overflows, and the sum is not finite exactly when some gradient
-// is not.  The order is the grid's, which the plan fixes: workgroup b sums a contiguous run of tiles.
+// is not.  The order is the grid's, which the plan fixes: workgroup b sums a contiguous run of tiles,
+// and one workgroup adds the sums -- in a launch of its own: counting arrivals at one address instead
+// took 10 ns for each workgroup, 36 with the cache's write-back, and 4.5 us in all is the launch.
+// A plan of at most kNormAlone tiles is one workgroup's, in one launch.
+constexpr int kNormAloneBlock = 1024;
+constexpr uint32_t kNormAlone = 32;
+
+template <int BS>
 __device__ __forceinline__ double block_sum(double x, double* lds) {
   for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
   __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  x = 0.0;
+#pragma unroll
+  for (int w = 0; w < BS / 64; w++) x += lds[w];
+  return x;
 }
 
-#ifndef NORM_U
-#define NORM_U 4
-#endif
+// The step's scalars from the sum of squares: three threads of different waves at once.  t: read from
+// ctrl by every thread before the barrier of the last sum.
+__device__ __forceinline__ void finish_norm(double sum, uint64_t t, const OptNorm& a, hydra_adamw_ctrl_t* c) {
+  const bool fine = sum < (double)INFINITY;
+  if (threadIdx.x == 0) {
+    const double norm = fabs(a.grad_scale) * sqrt(sum);
+    const double clip = a.max_norm > 0.0 ? fmin(1.0, a.max_norm / (norm + 1e-6)) : 1.0;
+    c->norm = (float)norm;
+    c->mult = (float)(a.grad_scale * clip);
+    c->skip = fine ? 0 : 1;
+    if (fine) c->step = (int64_t)t;
+    else c->skipped += 1;
+  } else if (threadIdx.x == 64 && fine) {
+    c->inv_bc1 = (float)(1.0 / (1.0 - power(a.beta1, t)));
+  } else if (threadIdx.x == 128 && fine) {
+    c->inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));
+  }
+}
+
 // the squares of a dword's gradients
 template <typename G>
 __device__ __forceinline__ void add_squares(uint32_t w, double& sum) {
@@ -496,16 +528,18 @@ __device__ __forceinline__ void add_squares(uint32_t w, double& sum) {
     sum = fma(b, b, sum);
   }
 }
-template <typename G>
-__global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* tensors,
-                                                            const uint32_t* tile_tensor,
-                                                            uint32_t tiles, uint64_t bucket,
-                                                            double* partials) {
-  constexpr int N = 16 / sizeof(G), U = NORM_U;  // elements of a 16-byte load, loads in flight
-  __shared__ double lds[4];
+
+// ALONE: the only workgroup, which finishes too
+template <typename G, int BS, bool ALONE>
+__global__ __launch_bounds__(BS) void k_norm(const OptTensor* tensors, const uint32_t* tile_tensor,
+                                             uint32_t each, uint32_t more, uint64_t bucket,
+                                             double* partials, OptNorm a, hydra_adamw_ctrl_t* ctrl) {
+  constexpr int N = 16 / sizeof(G), U = 2;  // elements of a 16-byte load, loads in flight
+  __shared__ double lds[BS / 64];
   const uint32_t b = xcd_tile(blockIdx.x, gridDim.x);
-  uint32_t tile = (uint32_t)((uint64_t)tiles * b / gridDim.x);
-  const uint32_t last = (uint32_t)((uint64_t)tiles * (b + 1) / gridDim.x);
+  uint32_t tile = b * each + min(b, more);  // the first `more` workgroups take one tile more
+  const uint32_t last = tile + each + (b < more ? 1u : 0u);
+  const uint64_t t = ALONE ? (uint64_t)ctrl->step + 1 : 0;
   double sum = 0.0;
   while (tile < last) {  // one tensor's share: [from, to)
     const OptTensor T = tensors[tile_tensor[tile]];
@@ -513,6 +547,7 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* ten
     const uint64_t from = first ? T.head + first * (uint64_t)kOptTile : 0;
     const uint64_t to = min(T.head + end * (uint64_t)kOptTile, T.n);
     const uint64_t addr = bucket + T.grad + from * sizeof(G), n = to - from;
+    // whole vectors from the first 16-byte boundary on; wave 0 takes what is before, wave 1 what is after
     const uint32_t head = (uint32_t)min((uint64_t)((16 - (addr & 15)) & 15) / sizeof(G), n);
     const uint64_t vecs = (n - head) / N;
     const uint32_t tail = (uint32_t)(n - head - vecs * N);
@@ -526,10 +561,10 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* ten
     }
     gptr at = ends + head * sizeof(G);
     uint64_t left = vecs;
-    for (; left >= kOptBlock * U; left -= kOptBlock * U, at += kOptBlock * U * 16) {
+    for (; left >= BS * U; left -= BS * U, at += BS * U * 16) {
       w4 x[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) x[u] = ldv<w4>(at, (u * kOptBlock + threadIdx.x) * 16);
+      for (int u = 0; u < U; u++) x[u] = ldv<w4>(at, (u * BS + threadIdx.x) * 16);
 #pragma unroll
       for (int u = 0; u < U; u++) {
 #pragma unroll
@@ -540,7 +575,7 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* ten
       w4 x[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const uint32_t v = u * kOptBlock + threadIdx.x;
+        const uint32_t v = u * BS + threadIdx.x;
         x[u] = w4{0, 0, 0, 0};
         if (v < left) x[u] = ldv<w4>(at, v * 16);
       }
@@ -552,34 +587,26 @@ __global__ __launch_bounds__(kOptBlock) void k_norm_partial(const OptTensor* ten
     }
     tile = T.tile0 + end;
   }
-  sum = block_sum(sum, lds);
-  if (threadIdx.x == 0) partials[b] = sum;
-}
-
-__device__ __forceinline__ void finish_norm(double sum, const OptNorm& a, hydra_adamw_ctrl_t* c) {
-  const double norm = fabs(a.grad_scale) * sqrt(sum);
-  const double clip = a.max_norm > 0.0 ? fmin(1.0, a.max_norm / (norm + 1e-6)) : 1.0;
-  c->norm = (float)norm;
-  c->mult = (float)(a.grad_scale * clip);
-  const bool fine = sum < (double)INFINITY;
-  c->skip = fine ? 0 : 1;
-  if (!fine) {
-    c->skipped += 1;
-    return;
-  }
-  const int64_t t = c->step + 1;
-  c->step = t;
-  c->inv_bc1 = (float)(1.0 / (1.0 - power(a.beta1, (uint64_t)t)));
-  c->inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - power(a.beta2, (uint64_t)t)));
+  sum = block_sum<BS>(sum, lds);
+  if constexpr (ALONE) finish_norm(sum, t, a, ctrl);
+  else if (threadIdx.x == 0) partials[b] = sum;
 }
 
 __global__ __launch_bounds__(kOptBlock) void k_norm_finish(const double* partials, uint32_t count,
                                                            OptNorm a, hydra_adamw_ctrl_t* ctrl) {
+  constexpr int U = kNormBlocks / kOptBlock;
   __shared__ double lds[4];
+  const uint64_t t = (uint64_t)ctrl->step + 1;
+  double x[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {  // all loads at once
+    const uint32_t j = u * kOptBlock + threadIdx.x;
+    x[u] = j < count ? partials[j] : 0.0;
+  }
   double sum = 0.0;
-  for (uint32_t j = threadIdx.x; j < count; j += kOptBlock) sum += partials[j];
-  sum = block_sum(sum, lds);
-  if (threadIdx.x == 0) finish_norm(sum, a, ctrl);
+#pragma unroll
+  for (int u = 0; u < U; u++) sum += x[u];
+  finish_norm(block_sum<kOptBlock>(sum, lds), t, a, ctrl);
 }
 
 // ---- 8-bit moments from and to values ---------------------------------------------------------------
@@ -589,7 +616,7 @@ constexpr size_t kConvTile = kOptBlock / 64 * 2 * kMomentBlock;  // elements of 
 // a wave's first element, and how many (up to 512) it has
 __device__ __forceinline__ uint32_t wave_part(size_t n, size_t* at) {
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  *at = (size_t)xcd_tile(blockIdx.x, gridDim.x) * kConvTile + wave * (2 * kMomentBlock);
+  *at = (size_t)blockIdx.x * kConvTile + wave * (2 * kMomentBlock);
   return *at < n ? (uint32_t)min(n - *at, (size_t)(2 * kMomentBlock)) : 0u;
 }
 __device__ __forceinline__ uint32_t rest(uint32_t left, uint32_t i) { return left > i ? left - i : 0u; }
@@ -619,7 +646,7 @@ __global__ __launch_bounds__(kOptBlock) void k_encode(uint8_t* m8, float* ms, ui
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       y[h][j] = fabsf(y[h][j]);
-      root[j] = __builtin_amdgcn_sqrtf(y[h][j]);
+      root[j] = plain_sqrt(y[h][j]);
       am = max(am, fbits(fabsf(x[h][j])));
       ar = max(ar, fbits(root[j]));
     }
@@ -719,7 +746,7 @@ hipError_t adamw_t(const OptTable& t, const OptStep& st, const void* bucket, hip
                        t.tile_tensor, t.tiles, st, reinterpret_cast<uint64_t>(bucket));
   else
     hipLaunchKernelGGL((k_adamw<P, G, MASTER>), dim3(t.tiles), dim3(kOptBlock), 0, s, t.tensors,
-                       t.tile_tensor, t.tiles, st, reinterpret_cast<uint64_t>(bucket));
+                       t.tile_tensor, st, reinterpret_cast<uint64_t>(bucket));
   return hipGetLastError();
 }
 
@@ -750,10 +777,21 @@ hipError_t adamw_p(const hydra_adamw_config_t& c, const OptTable& t, const OptSt
 }
 
 template <typename G>
-void norm_partial(const OptTable& t, const void* bucket, double* partials, hipStream_t s) {
-  hipLaunchKernelGGL((k_norm_partial<G>), dim3(norm_partials(t.tiles)), dim3(kOptBlock), 0, s,
-                     t.tensors, t.tile_tensor, t.tiles, reinterpret_cast<uint64_t>(bucket),
-                     partials);
+hipError_t norm_t(const OptTable& t, const OptNorm& norm, const void* bucket,
+                  hydra_adamw_ctrl_t* ctrl, double* partials, hipStream_t s) {
+  const uint64_t at = reinterpret_cast<uint64_t>(bucket);
+  if (t.tiles <= kNormAlone) {
+    hipLaunchKernelGGL((k_norm<G, kNormAloneBlock, true>), dim3(1), dim3(kNormAloneBlock), 0, s,
+                       t.tensors, t.tile_tensor, t.tiles, 0u, at, partials, norm, ctrl);
+    return hipGetLastError();
+  }
+  const uint32_t blocks = std::min(t.tiles, (uint32_t)kNormBlocks);
+  hipLaunchKernelGGL((k_norm<G, kOptBlock, false>), dim3(blocks), dim3(kOptBlock), 0, s, t.tensors,
+                     t.tile_tensor, t.tiles / blocks, t.tiles % blocks, at, partials, norm, ctrl);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(kOptBlock), 0, s, partials, blocks, norm, ctrl);
+  return hipGetLastError();
 }
 
 constexpr size_t kPart = size_t(1) << 30;  // elements of one launch, whole blocks
@@ -799,22 +837,19 @@ hipError_t launch_adamw(const hydra_adamw_config_t& cfg, const OptTable& t, cons
                                         : adamw_p<false>(cfg, t, st, bucket, s);
 }
 
-uint32_t norm_partials(uint32_t tiles) { return std::max(1u, std::min(tiles, (uint32_t)kNormBlocks)); }
+size_t norm_workspace(uint32_t tiles) {
+  return tiles <= kNormAlone ? 0 : std::min(tiles, (uint32_t)kNormBlocks) * sizeof(double);
+}
 
 hipError_t launch_grad_norm(int grad_dtype, const OptTable& t, const OptNorm& norm,
                             const void* bucket, hydra_adamw_ctrl_t* ctrl, double* partials,
                             hipStream_t s) {
   switch (grad_dtype) {
-    case HYDRA_FLOAT32: norm_partial<float>(t, bucket, partials, s); break;
-    case HYDRA_BFLOAT16: norm_partial<bf16_t>(t, bucket, partials, s); break;
-    case HYDRA_FLOAT16: norm_partial<f16_t>(t, bucket, partials, s); break;
-    default: return hipErrorInvalidValue;
+    case HYDRA_FLOAT32: return norm_t<float>(t, norm, bucket, ctrl, partials, s);
+    case HYDRA_BFLOAT16: return norm_t<bf16_t>(t, norm, bucket, ctrl, partials, s);
+    case HYDRA_FLOAT16: return norm_t<f16_t>(t, norm, bucket, ctrl, partials, s);
   }
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(kOptBlock), 0, s, partials,
-                     norm_partials(t.tiles), norm, ctrl);
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 hipError_t launch_moments8_encode(int dtype, uint8_t* m8, float* ms, uint8_t* v8, float* vs,

@@ -22,12 +22,18 @@ from __future__ import annotations
 import ctypes
 import sys
 
+import torch
+
 from . import _lib
 from ._lib import HydraError, check
 
 _is_finalizing = sys.is_finalizing
 
 MOMENT_BLOCK = 256  # elements that share one scale of an 8-bit moment
+_CODES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
+# the current stream's handle by device index (torch.cuda.current_stream builds a Stream object
+# around it: 2 us, as long as a small step's kernel runs)
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def moment_scales(n: int) -> int:
@@ -36,18 +42,13 @@ def moment_scales(n: int) -> int:
 
 
 def _code(dtype) -> int:
-    import torch
-
-    codes = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
     try:
-        return codes[dtype]
+        return _CODES[dtype]
     except KeyError:
         raise HydraError(_lib.ERR_INVALID, f"unsupported dtype {dtype}") from None
 
 
 def _list(x) -> list:
-    import torch
-
     return [x] if isinstance(x, torch.Tensor) else list(x)
 
 
@@ -61,11 +62,10 @@ class Control:
     program (ctrl.lr.fill_(x)), the others are written by grad_norm_."""
 
     def __init__(self, device, lr: float = 0.0, step: int = 0):
-        import torch
-
         self.buffer = torch.zeros(64, dtype=torch.uint8, device=device)
         if not self.buffer.is_cuda:
             _refuse("Control: a GPU device is required")
+        self.index, self.ptr = self.buffer.get_device(), self.buffer.data_ptr()
         f, i = self.buffer.view(torch.float32), self.buffer.view(torch.int32)
         self.step, self.skipped = self.buffer.view(torch.int64)[:2]
         self.lr, self.mult, self.norm = f[4], f[5], f[6]
@@ -88,8 +88,6 @@ class AdamW:
     def __init__(self, params, grads, m=None, v=None, *, master=None, m_scale=None, v_scale=None,
                  betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0,
                  bucket=None):
-        import torch
-
         self._h = ctypes.c_void_p()
         grads = _list(grads)
         if not grads:
@@ -143,7 +141,8 @@ class AdamW:
                 end = g.data_ptr() + g.numel() * g.element_size()
                 if g.numel() and not (base <= g.data_ptr() and end <= base + self._bucket_bytes):
                     _refuse("AdamW: a grad is not a view of the bucket")
-        self.device, self._grad_dtype, self._bucket = device, grads[0].dtype, bucket
+        self.device, self._index = device, grads[0].get_device()
+        self._grad_dtype, self._bucket = grads[0].dtype, bucket
         # what the launches touch; with buckets of the caller's choice, not the first one's views
         self._keep = [*lists.values(), grads if bucket is None else ()]
         ptr = lambda name, i: lists[name][i].data_ptr() if name in lists else None  # noqa: E731
@@ -160,7 +159,7 @@ class AdamW:
                                _code(self._grad_dtype),
                                _lib.UINT8 if eight else _lib.FLOAT32, flags, betas[0], betas[1], eps)
         L = _lib.lib()
-        check(L.hydra_adamw_create(device.index, ctypes.byref(cfg), ts, k, ctypes.byref(self._h)))
+        check(L.hydra_adamw_create(self._index, ctypes.byref(cfg), ts, k, ctypes.byref(self._h)))
         size = ctypes.c_size_t()
         check(L.hydra_adamw_workspace(self._h, ctypes.byref(size)))
         self._workspace = size.value
@@ -192,35 +191,32 @@ class AdamW:
                    stream: int | None = None) -> None:
         """hydra_adamw_grad_norm: norm, clip factor and finite check of all gradients into ctrl, and
         the next step's number.  max_norm 0: no clipping."""
-        import torch
-
         h, b = self._handle(), self._bucket_ptr(bucket)
-        if ctrl.buffer.device != self.device:
+        if ctrl.index != self._index:
             _refuse("grad_norm_: ctrl is on another device")
-        with torch.cuda.device(self.device):
-            s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
-            ws = torch.empty(self._workspace, dtype=torch.uint8, device=self.device)
-            if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
-                ws.record_stream(torch.cuda.ExternalStream(stream))
-            check(_lib.lib().hydra_adamw_grad_norm(h, b, grad_scale, max_norm,
-                                                   ctrl.buffer.data_ptr(), ws.data_ptr(),
-                                                   self._workspace, s))
+        s, ws, size = stream, None, self._workspace
+        if stream is None:
+            s = _current_stream(self._index)
+        if size:  # from torch's allocator, for this call: two graphs of one plan share none
+            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            if stream is not None and stream != _current_stream(self._index):
+                ws.record_stream(torch.cuda.ExternalStream(stream, device=self.device))
+            ws = ws.data_ptr()
+        check(_lib.lib().hydra_adamw_grad_norm(h, b, grad_scale, max_norm, ctrl.ptr, ws, size, s))
 
     def step_(self, lr: float | None = None, step: int | None = None, grad_scale: float = 1.0,
               ctrl: Control | None = None, seed: int = 0, bucket=None,
               stream: int | None = None) -> None:
         """One AdamW step in place: with lr and step (1, 2, ...) from the arguments, or with ctrl
         from the last grad_norm_ on it.  seed: that of the 8-bit moments' rounding (0: to nearest)."""
-        import torch
-
         h, b = self._handle(), self._bucket_ptr(bucket)
-        s = stream if stream is not None else torch.cuda.current_stream(self.device).cuda_stream
+        s = stream if stream is not None else _current_stream(self._index)
         if ctrl is not None:
             if lr is not None or step is not None or grad_scale != 1.0:
                 _refuse("step_: lr, step and grad_scale come from ctrl")
-            if ctrl.buffer.device != self.device:
+            if ctrl.index != self._index:
                 _refuse("step_: ctrl is on another device")
-            check(_lib.lib().hydra_adamw_step_ctrl(h, b, ctrl.buffer.data_ptr(), seed, s))
+            check(_lib.lib().hydra_adamw_step_ctrl(h, b, ctrl.ptr, seed, s))
             return
         if lr is None or step is None:
             _refuse("step_: lr and step, or ctrl")
@@ -234,7 +230,8 @@ class AdamW:
             self._keep = []
 
     def __del__(self):
-        if _is_finalizing():  # no HIP calls while the interpreter is finalizing
+        # no HIP calls while the interpreter is finalizing (this module's names may be gone by then)
+        if _is_finalizing is None or _is_finalizing():
             return
         try:
             self.close()
@@ -243,49 +240,44 @@ class AdamW:
 
 
 def _moments(m, v, m8, m_scale, v8, v_scale):
-    """Checks a conversion's tensors; (device, dtype code, n, pointers by name)."""
-    import torch
-
-    if m is None and v is None:
+    """Checks a conversion's tensors; (device index, dtype code, n, m's pointers, v's)."""
+    some = m if m is not None else v
+    if some is None:
         _refuse("moments8: neither moment given")
-    n = (m if m is not None else v).numel()
-    ptrs, values = {}, [t for t in (m, v) if t is not None]
+    n, dtype, index = some.numel(), some.dtype, some.get_device()
+    if index < 0:
+        _refuse("moments8: contiguous tensors on one GPU are required")
+    pointers = []
     for x, codes, scale, name in ((m, m8, m_scale, "m"), (v, v8, v_scale, "v")):
         if x is None:
             if codes is not None or scale is not None:
                 _refuse(f"moments8: codes or scales of {name} without its values")
-            ptrs[name] = (None, None, None)
+            pointers.append((None, None, None))
             continue
         if codes is None or scale is None:
             _refuse(f"moments8: {name} needs its codes and its scales")
         for t in (x, codes, scale):
-            if not t.is_cuda or t.device != values[0].device or not t.is_contiguous():
+            if t.get_device() != index or not t.is_contiguous():
                 _refuse("moments8: contiguous tensors on one GPU are required")
-        if codes.dtype != torch.uint8 or scale.dtype != torch.float32 or x.dtype != values[0].dtype:
+        if codes.dtype != torch.uint8 or scale.dtype != torch.float32 or x.dtype != dtype:
             _refuse("moments8: uint8 codes, float32 scales and values of one dtype are required")
         if x.numel() != n or codes.numel() != n or scale.numel() != moment_scales(n):
             _refuse(f"moments8: {name}: lengths do not fit {n} elements")
-        ptrs[name] = (x.data_ptr(), codes.data_ptr(), scale.data_ptr())
-    return values[0].device, _code(values[0].dtype), n, ptrs
+        pointers.append((x.data_ptr(), codes.data_ptr(), scale.data_ptr()))
+    return index, _code(dtype), n, *pointers
 
 
 def moments8_encode_(m8, m_scale, v8, v_scale, m, v, stream: int | None = None) -> None:
     """One tensor's moments (fp32 or bf16) into 8 bits, to nearest; either moment may be None."""
-    import torch
-
-    dev, code, n, p = _moments(m, v, m8, m_scale, v8, v_scale)
-    with torch.cuda.device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
-        check(_lib.lib().hydra_moments8_encode(p["m"][1], p["m"][2], p["v"][1], p["v"][2],
-                                               p["m"][0], p["v"][0], code, n, s))
+    index, code, n, pm, pv = _moments(m, v, m8, m_scale, v8, v_scale)
+    with torch.cuda.device(index):
+        s = stream if stream is not None else _current_stream(index)
+        check(_lib.lib().hydra_moments8_encode(pm[1], pm[2], pv[1], pv[2], pm[0], pv[0], code, n, s))
 
 
 def moments8_decode_(m, v, m8, m_scale, v8, v_scale, stream: int | None = None) -> None:
     """The values that 8-bit moments stand for, into fp32 or bf16; either moment may be None."""
-    import torch
-
-    dev, code, n, p = _moments(m, v, m8, m_scale, v8, v_scale)
-    with torch.cuda.device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream().cuda_stream
-        check(_lib.lib().hydra_moments8_decode(p["m"][0], p["v"][0], code, p["m"][1], p["m"][2],
-                                               p["v"][1], p["v"][2], n, s))
+    index, code, n, pm, pv = _moments(m, v, m8, m_scale, v8, v_scale)
+    with torch.cuda.device(index):
+        s = stream if stream is not None else _current_stream(index)
+        check(_lib.lib().hydra_moments8_decode(pm[0], pv[0], code, pm[1], pm[2], pv[1], pv[2], n, s))

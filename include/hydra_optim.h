@@ -106,8 +106,8 @@ int hydra_adamw_destroy(hydra_adamw_t plan);
  * the same bits on every call and on every rank that holds the same bits.  max_norm > 0 clips:
  * mult = grad_scale * min(1, max_norm / (norm + 1e-6)); 0: mult = grad_scale.  If the sum is not
  * finite, skip = 1 and skipped += 1; else step += 1 and the fields for that step are set.
- * workspace: hydra_adamw_workspace() bytes of device memory, 8-byte aligned, needed until the
- * call has run; its contents do not matter. */
+ * workspace: hydra_adamw_workspace() bytes of device memory (none for a small plan: NULL then),
+ * 8-byte aligned, needed until the call has run; its contents do not matter. */
 int hydra_adamw_workspace(hydra_adamw_t plan, size_t* bytes);
 int hydra_adamw_grad_norm(hydra_adamw_t plan, const void* bucket, double grad_scale,
                           double max_norm, hydra_adamw_ctrl_t* ctrl, void* workspace,

@@ -12,7 +12,7 @@ namespace hydra {
 constexpr int kOptBlock = 256;      // 4 waves of 64 lanes
 constexpr int kMomentBlock = 256;   // elements that share one scale of an 8-bit moment
 constexpr size_t kOptTile = 1024;   // elements of one tensor that a workgroup takes
-constexpr int kNormBlocks = 1024;   // workgroups (and partial sums) of the norm, at most
+constexpr int kNormBlocks = 2048;   // workgroups (and partial sums) of the norm, at most
 
 // One tensor of a plan, in device memory.  `grad` counts from the bucket that a call gives (null:
 // an address).  Its tile k is number tile0 + k and holds the elements [head + k * kOptTile,

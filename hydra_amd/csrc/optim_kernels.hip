@@ -146,6 +146,8 @@ template <> struct At<f16_t> {
 // bytes
 __device__ __forceinline__ uint32_t load_byte(gptr p, uint32_t i) { return *(const GLOBAL uint8_t*)(p + i); }
 __device__ __forceinline__ void store_byte(gptr p, uint32_t i, uint32_t x) { *(GLOBAL uint8_t*)(p + i) = (uint8_t)x; }
+// elements from i on
+__device__ __forceinline__ uint32_t rest(uint32_t left, uint32_t i) { return left > i ? left - i : 0u; }
 // the first `count` (0 to 4) of four
 template <typename E>
 __device__ __forceinline__ f4 load_upto4(gptr p, uint32_t i, uint32_t count) {
@@ -366,13 +368,25 @@ __device__ __forceinline__ float uniform(float x, int lane) {
 // does not see, and the quotient is a product with the hardware's reciprocal (2 ulp).
 template <typename P, typename G, bool MASTER>
 __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr m8, gptr v8,
-                                       gptr ms, gptr vs, uint32_t count, uint32_t lane,
+                                       gptr ms, gptr vs, uint32_t left, uint32_t lane,
                                        uint32_t rnd, uint32_t rkey, const Scalars& k) {
-  // the pointers are the block's; count: elements from this lane's first one to the tensor's end
+  // the pointers are the block's; left: elements from there to the tensor's end
+  const bool whole = left >= kMomentBlock;
+  const uint32_t count = rest(left, lane * 4);
   const uint32_t i = lane * 4;
-  f4 p = MASTER ? load_upto4<float>(master, i, count) : load_upto4<P>(param, i, count);
-  const f4 g = load_upto4<G>(grad, i, count);
-  const uint32_t cm = load_bytes(m8, i, count), cv = load_bytes(v8, i, count);
+  f4 p, g;
+  uint32_t cm, cv;
+  if (whole) {
+    p = MASTER ? At<float>::wide(At<float>::load4(master, i)) : At<P>::wide(At<P>::load4(param, i));
+    g = At<G>::wide(At<G>::load4(grad, i));
+    cm = ldv<w1>(m8, i);
+    cv = ldv<w1>(v8, i);
+  } else {
+    p = MASTER ? load_upto4<float>(master, i, count) : load_upto4<P>(param, i, count);
+    g = load_upto4<G>(grad, i, count);
+    cm = load_bytes(m8, i, count);
+    cv = load_bytes(v8, i, count);
+  }
   const float ms0 = At<float>::load(ms, 0), vs0 = At<float>::load(vs, 0);
   f4 m, v, root;
   const bool odd = !(ms0 < 0x1p15f && vs0 < 0x1p15f) ||
@@ -443,10 +457,17 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
     }
   }
   if ((lane & 31) == 31) At<float>::store(lane & 32 ? vs : ms, 0, scale);
-  if (MASTER) store_upto4<float>(master, i, p, count);
-  store_upto4<P>(param, i, p, count);
-  store_bytes(m8, i, wm, count);
-  store_bytes(v8, i, wv, count);
+  if (whole) {
+    if (MASTER) At<float>::store4(master, i, p);
+    At<P>::store4(param, i, p);
+    store_bytes(m8, i, wm, 4);
+    store_bytes(v8, i, wv, 4);
+  } else {
+    if (MASTER) store_upto4<float>(master, i, p, count);
+    store_upto4<P>(param, i, p, count);
+    store_bytes(m8, i, wm, count);
+    store_bytes(v8, i, wv, count);
+  }
 }
 
 template <typename P, typename G, bool MASTER>
@@ -464,7 +485,6 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
   const uint32_t i0 = wave * kMomentBlock;
   if (i0 >= left) return;  // whole waves
   const uint64_t at = base + i0;  // the wave's block
-  const uint32_t count = left - i0 > lane * 4 ? left - i0 - lane * 4 : 0u;
   const uint32_t rnd = ((uint32_t)at + lane * 4) * 0x9E3779B1u;
   const uint32_t rkey = k.key ^ ((uint32_t)(at >> 32) * 0x85EBCA6Bu);
   const gptr master = global(T.master) + at * 4, param = global(T.param) + at * sizeof(P);
@@ -472,7 +492,7 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
   const gptr m8 = global(T.m) + at, v8 = global(T.v) + at;
   const gptr ms = global(T.m_scale) + at / kMomentBlock * 4;
   const gptr vs = global(T.v_scale) + at / kMomentBlock * 4;
-  block8<P, G, MASTER>(master, param, grad, m8, v8, ms, vs, count, lane, rnd, rkey, k);
+  block8<P, G, MASTER>(master, param, grad, m8, v8, ms, vs, left - i0, lane, rnd, rkey, k);
 }
 
 // ---- the norm --------------------------------------------------------------------------------------
@@ -529,14 +549,22 @@ __device__ __forceinline__ void add_squares(uint32_t w, double& sum) {
   }
 }
 
+// the thread's vector of `left` ones
+template <int BS>
+__device__ __forceinline__ w4 vector_or_zero(gptr at, uint64_t left) {
+  w4 x = {0, 0, 0, 0};
+  if (threadIdx.x < left) x = ldv<w4>(at, threadIdx.x * 16);
+  return x;
+}
+
 // ALONE: the only workgroup, which finishes too
 template <typename G, int BS, bool ALONE>
 __global__ __launch_bounds__(BS) void k_norm(const OptTensor* tensors, const uint32_t* tile_tensor,
                                              uint32_t each, uint32_t more, uint64_t bucket,
                                              double* partials, OptNorm a, hydra_adamw_ctrl_t* ctrl) {
-  constexpr int N = 16 / sizeof(G), U = 2;  // elements of a 16-byte load, loads in flight
+  constexpr int N = 16 / sizeof(G);  // elements of a vector
   __shared__ double lds[BS / 64];
-  const uint32_t b = xcd_tile(blockIdx.x, gridDim.x);
+  const uint32_t b = blockIdx.x;
   uint32_t tile = b * each + min(b, more);  // the first `more` workgroups take one tile more
   const uint32_t last = tile + each + (b < more ? 1u : 0u);
   const uint64_t t = ALONE ? (uint64_t)ctrl->step + 1 : 0;
@@ -560,30 +588,16 @@ __global__ __launch_bounds__(BS) void k_norm(const OptTensor* tensors, const uin
       sum = fma(g, g, sum);
     }
     gptr at = ends + head * sizeof(G);
-    uint64_t left = vecs;
-    for (; left >= BS * U; left -= BS * U, at += BS * U * 16) {
-      w4 x[U];
+    // one vector per thread and turn, the next one's load in flight while this one is summed
+    w4 x = vector_or_zero<BS>(at, vecs);
+    for (uint64_t left = vecs; left;) {
+      const uint64_t next = left > BS ? left - BS : 0;
+      at += BS * 16;
+      const w4 y = vector_or_zero<BS>(at, next);
 #pragma unroll
-      for (int u = 0; u < U; u++) x[u] = ldv<w4>(at, (u * BS + threadIdx.x) * 16);
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) add_squares<G>(x[u][j], sum);
-      }
-    }
-    if (left) {  // the last turn: vectors that are not there count as zeros
-      w4 x[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const uint32_t v = u * BS + threadIdx.x;
-        x[u] = w4{0, 0, 0, 0};
-        if (v < left) x[u] = ldv<w4>(at, v * 16);
-      }
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) add_squares<G>(x[u][j], sum);
-      }
+      for (int j = 0; j < 4; j++) add_squares<G>(x[j], sum);
+      x = y;
+      left = next;
     }
     tile = T.tile0 + end;
   }
@@ -619,7 +633,6 @@ __device__ __forceinline__ uint32_t wave_part(size_t n, size_t* at) {
   *at = (size_t)blockIdx.x * kConvTile + wave * (2 * kMomentBlock);
   return *at < n ? (uint32_t)min(n - *at, (size_t)(2 * kMomentBlock)) : 0u;
 }
-__device__ __forceinline__ uint32_t rest(uint32_t left, uint32_t i) { return left > i ? left - i : 0u; }
 
 // encode: 4 elements per lane of each block, all loads first (8 consecutive ones per lane leave every
 // fp32 load half of the lines it touches)

@@ -394,7 +394,7 @@ int hydra_adamw_grad_norm(hydra_adamw_t plan, const void* bucket, double grad_sc
   HIP_TRY(ds.err);
   const hydra::OptNorm norm{grad_scale, max_norm, plan->cfg.beta1, plan->cfg.beta2};
   const hipError_t e =
-      hydra::launch_grad_norm(plan->cfg.grad_dtype, plan->table, norm, bucket, ctrl,
+      hydra::launch_grad_norm(plan->cfg, plan->table, norm, bucket, ctrl,
                               static_cast<double*>(workspace), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "gradient norm kernel launch");
   return ok();

@@ -73,7 +73,7 @@ __host__ __device__ inline double power(double beta, uint64_t t) {
 hipError_t launch_adamw(const hydra_adamw_config_t& cfg, const OptTable& t, const OptStep& step,
                         const void* bucket, hipStream_t s);
 size_t norm_workspace(uint32_t tiles);  // bytes of partial sums
-hipError_t launch_grad_norm(int grad_dtype, const OptTable& t, const OptNorm& norm,
+hipError_t launch_grad_norm(const hydra_adamw_config_t& cfg, const OptTable& t, const OptNorm& norm,
                             const void* bucket, hydra_adamw_ctrl_t* ctrl, double* partials,
                             hipStream_t s);
 hipError_t launch_moments8_encode(int dtype, uint8_t* m8, float* m_scale, uint8_t* v8,

@@ -96,6 +96,10 @@ class AdamWTensor(ctypes.Structure):
                 ("weight_decay", ctypes.c_float)]
 
 
+# the same layout as a numpy record, to fill a long list of tensors by columns
+ADAMW_TENSOR = [(name, "<f4" if t is ctypes.c_float else "<u8") for name, t in AdamWTensor._fields_]
+
+
 class AdamWConfig(ctypes.Structure):
     """hydra_adamw_config_t (include/hydra_optim.h)."""
     _fields_ = [("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32),
@@ -277,8 +281,7 @@ def _declare(L) -> None:
     L.hydra_test_set.argtypes = [i, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)]
     L.hydra_test_get.argtypes = [i, ctypes.POINTER(ctypes.c_int64)]
     u64, dbl = ctypes.c_uint64, ctypes.c_double
-    L.hydra_adamw_create.argtypes = [i, ctypes.POINTER(AdamWConfig), ctypes.POINTER(AdamWTensor), sz,
-                                     ctypes.POINTER(vp)]
+    L.hydra_adamw_create.argtypes = [i, ctypes.POINTER(AdamWConfig), vp, sz, ctypes.POINTER(vp)]
     L.hydra_adamw_destroy.argtypes = [vp]
     L.hydra_adamw_workspace.argtypes = [vp, ctypes.POINTER(sz)]
     L.hydra_adamw_grad_norm.argtypes = [vp, vp, dbl, dbl, vp, vp, sz, vp]

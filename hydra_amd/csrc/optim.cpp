@@ -52,17 +52,25 @@ bool float_dtype(int d) {
 
 bool aligned(const void* p, size_t es) { return reinterpret_cast<uintptr_t>(p) % es == 0; }
 
-// the first and the last byte of a range are memory of `device`
-bool on_device(uintptr_t lo, uintptr_t hi, int device) {
-  for (uintptr_t p : {lo, hi - 1}) {
-    hipPointerAttribute_t a{};
-    if (hipPointerGetAttributes(&a, reinterpret_cast<const void*>(p)) != hipSuccess) {
-      (void)hipGetLastError();
-      return false;
-    }
-    if ((a.type != hipMemoryTypeDevice && a.type != hipMemoryTypeManaged) || a.device != device)
-      return false;
+bool byte_on_device(uintptr_t p, int device) {
+  hipPointerAttribute_t a{};
+  if (hipPointerGetAttributes(&a, reinterpret_cast<const void*>(p)) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
   }
+  return (a.type == hipMemoryTypeDevice || a.type == hipMemoryTypeManaged) && a.device == device;
+}
+// The first and the last byte of r are memory of `device`.  `known`: the allocation that the last
+// query found, which holds most of the ranges that follow (views of a few buffers).
+bool on_device(const Range& r, int device, Range* known) {
+  if (known->lo <= r.lo && r.hi <= known->hi) return true;
+  if (!byte_on_device(r.lo, device) || !byte_on_device(r.hi - 1, device)) return false;
+  hipDeviceptr_t base = nullptr;
+  size_t bytes = 0;
+  if (hipMemGetAddressRange(&base, &bytes, reinterpret_cast<hipDeviceptr_t>(r.lo)) == hipSuccess)
+    *known = {reinterpret_cast<uintptr_t>(base), reinterpret_cast<uintptr_t>(base) + bytes};
+  else
+    (void)hipGetLastError();  // (memory mapped by its owner: asked for range by range)
   return true;
 }
 
@@ -194,12 +202,13 @@ int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_ten
   if (device < 0 || device >= devices) return fail(HYDRA_ERR_NO_DEVICE, "no such device");
   hydra::DeviceScope ds(device);
   HIP_TRY(ds.err);
+  Range known{0, 0};
   for (const Range& r : written)
-    if (!on_device(r.lo, r.hi, device))
+    if (!on_device(r, device, &known))
       return fail(HYDRA_ERR_INVALID, "a param, master or moment is not memory of the plan's device");
   if (!bucket)
     for (const Range& r : grads)
-      if (!on_device(r.lo, r.hi, device))
+      if (!on_device(r, device, &known))
         return fail(HYDRA_ERR_INVALID, "a gradient is not memory of the plan's device");
 
   hydra_adamw& P = **made;
@@ -259,7 +268,8 @@ int check_bucket(const hydra_adamw& P, const void* bucket) {
   const Range r{b + P.bucket_lo, b + P.bucket_hi};
   if (touches(P.written, r))
     return fail(HYDRA_ERR_INVALID, "the bucket overlaps what the step writes");
-  if (!on_device(r.lo, r.hi, P.device))
+  Range known{0, 0};
+  if (!on_device(r, P.device, &known))
     return fail(HYDRA_ERR_INVALID, "the bucket is not memory of the plan's device");
   return HYDRA_OK;
 }

@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import sys
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -100,16 +101,17 @@ class AdamW:
         if not norm_only and (m is None or v is None):
             _refuse("AdamW: m and v are required")
         lists = {name: _list(x) for name, x in lists.items() if x is not None}
-        device = grads[0].device
+        index = grads[0].get_device()
         for name, ts in [("grads", grads), *lists.items()]:
             if len(ts) != k:
                 _refuse(f"AdamW: {len(ts)} {name} for {k} grads")
+            dtype = ts[0].dtype
             for t in ts:
-                if not t.is_cuda or t.device != device:
+                if t.get_device() != index or index < 0:
                     _refuse(f"AdamW: {name} must be on one GPU, that of the grads")
                 if not t.is_contiguous():
                     _refuse(f"AdamW: {name} must be contiguous")
-                if t.dtype != ts[0].dtype:
+                if t.dtype != dtype:
                     _refuse(f"AdamW: {name} must share one dtype")
         eight = not norm_only and lists["m"][0].dtype == torch.uint8
         if not norm_only:
@@ -121,11 +123,13 @@ class AdamW:
             for name in ("master", "m_scale", "v_scale"):
                 if name in lists and lists[name][0].dtype != torch.float32:
                     _refuse(f"AdamW: {name} must be float32")
+        sizes = [g.numel() for g in grads]
+        rows = [moment_scales(n) for n in sizes] if eight else None
         for name, ts in lists.items():
-            for t, g in zip(ts, grads):
-                want = moment_scales(g.numel()) if name.endswith("_scale") else g.numel()
-                if t.numel() != want:
-                    _refuse(f"AdamW: {name} of {t.numel()} elements where {want} are needed")
+            have, want = [t.numel() for t in ts], rows if name.endswith("_scale") else sizes
+            if have != want:
+                i = next(i for i in range(k) if have[i] != want[i])
+                _refuse(f"AdamW: {name} of {have[i]} elements where {want[i]} are needed")
         wd = list(weight_decay) if hasattr(weight_decay, "__iter__") else [weight_decay] * k
         ls = list(lr_scale) if hasattr(lr_scale, "__iter__") else [lr_scale] * k
         if len(wd) != k or len(ls) != k:
@@ -141,17 +145,16 @@ class AdamW:
                 end = g.data_ptr() + g.numel() * g.element_size()
                 if g.numel() and not (base <= g.data_ptr() and end <= base + self._bucket_bytes):
                     _refuse("AdamW: a grad is not a view of the bucket")
-        self.device, self._index = device, grads[0].get_device()
+        self.device, self._index = grads[0].device, index
         self._grad_dtype, self._bucket = grads[0].dtype, bucket
         # what the launches touch; with buckets of the caller's choice, not the first one's views
         self._keep = [*lists.values(), grads if bucket is None else ()]
-        ptr = lambda name, i: lists[name][i].data_ptr() if name in lists else None  # noqa: E731
-        ts = (_lib.AdamWTensor * k)()
-        for i, g in enumerate(grads):
-            ts[i] = _lib.AdamWTensor(ptr("params", i), ptr("master", i),
-                                     g.data_ptr() - base if g.numel() else 0, ptr("m", i),
-                                     ptr("v", i), ptr("m_scale", i), ptr("v_scale", i), g.numel(),
-                                     ls[i], wd[i])
+        table = np.zeros(k, _lib.ADAMW_TENSOR)
+        columns = {"params": "param"}
+        for name, ts in lists.items():
+            table[columns.get(name, name)] = [t.data_ptr() for t in ts]
+        table["grad"] = [g.data_ptr() - base if n else 0 for g, n in zip(grads, sizes)]
+        table["n"], table["lr_scale"], table["weight_decay"] = sizes, ls, wd
         flags = (_lib.ADAMW_MASTER if master is not None else 0) | \
                 (_lib.ADAMW_BUCKET if bucket is not None else 0) | \
                 (_lib.ADAMW_NORM_ONLY if norm_only else 0)
@@ -159,7 +162,8 @@ class AdamW:
                                _code(self._grad_dtype),
                                _lib.UINT8 if eight else _lib.FLOAT32, flags, betas[0], betas[1], eps)
         L = _lib.lib()
-        check(L.hydra_adamw_create(self._index, ctypes.byref(cfg), ts, k, ctypes.byref(self._h)))
+        check(L.hydra_adamw_create(self._index, ctypes.byref(cfg), table.ctypes.data, k,
+                                   ctypes.byref(self._h)))
         size = ctypes.c_size_t()
         check(L.hydra_adamw_workspace(self._h, ctypes.byref(size)))
         self._workspace = size.value

@@ -4,8 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstring>
-#include <new>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -268,8 +267,7 @@ int check_bucket(const hydra_adamw& P, const void* bucket) {
   const Range r{b + P.bucket_lo, b + P.bucket_hi};
   if (touches(P.written, r))
     return fail(HYDRA_ERR_INVALID, "the bucket overlaps what the step writes");
-  Range known{0, 0};
-  if (!on_device(r, P.device, &known))
+  if (!byte_on_device(r.lo, P.device) || !byte_on_device(r.hi - 1, P.device))
     return fail(HYDRA_ERR_INVALID, "the bucket is not memory of the plan's device");
   return HYDRA_OK;
 }
@@ -356,8 +354,8 @@ int hydra_adamw_create(int device, const hydra_adamw_config_t* config,
   try {
     plan = new hydra_adamw;
     rc = create(device, config, tensors, count, &plan);
-  } catch (const std::bad_alloc&) {
-    rc = fail(HYDRA_ERR_HIP, "hydra_adamw_create: out of host memory");
+  } catch (const std::exception& e) {  // (of the vectors: out of host memory)
+    rc = fail(HYDRA_ERR_HIP, std::string("hydra_adamw_create: ") + e.what());
   }
   if (rc) {
     if (plan && plan->block) (void)hydra::cached_free(plan->block);

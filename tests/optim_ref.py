@@ -50,7 +50,10 @@ def step64(p, g, m, v, *, lr, t, mult=1.0, b1=0.9, b2=0.999, eps=1e-8, wd=0.0):
     with np.errstate(invalid="ignore", divide="ignore"):
         denom = np.sqrt(v1) * c2 + eps
         u = m1 / denom * (lr * c1)
-        eu = em / denom * (lr * c1)
+        # a v below 2^-126 is held in steps of 2^-149: three roundings (two products, the sum) of half
+        # a step, and its old value's; half of their share in v is the root's
+        coarse = np.where(v1 > 0, np.minimum(2.0 ** -148 / (2 * v1), 1.0), 0.0) * np.sqrt(v1) * c2 / denom
+        eu = em / denom * (lr * c1) + np.abs(u) * np.where(denom > 0, coarse, 0.0)
     p1 = p * (1 - lr * wd) - u
     ep = U32 * (np.abs(p) * (2 + 5 * abs(lr * wd)) + 16 * np.abs(u) + np.abs(p1)) + 2 * eu + 2.0 ** -149
     return (p1, m1, v1), (ep, em, ev)
@@ -133,8 +136,36 @@ def check_codes(x, ex, codes, scales, bits, noise, where="", loose=1e-3):
         lo, hi = np.maximum(lo, least), np.maximum(hi, least)
     wrong = (got < lo) | (got > hi)
     assert not wrong.any(), (where, int(wrong.sum()), a[wrong][:4], got[wrong][:4], lo[wrong][:4], hi[wrong][:4])
-    # the intervals are narrow: almost every byte is pinned to one value
-    assert n < 1000 or (lo != hi).mean() < loose, where
+    # the intervals are narrow: almost every byte is pinned to one value (counted where fp32 has the
+    # value to 2^-19: what comes from a v below 2^-126, held in steps of 2^-149, has a wide one)
+    sure = e <= 2.0 ** -19 * a
+    assert sure.sum() < 1000 or (lo != hi)[sure].mean() < loose, where
+
+
+def encode32(m, v, r):
+    """Bytes and scales of both moments from fp32 ones, operation by operation: (m codes, m scales, v
+    codes, v scales, which bytes are above the gradual underflow).  All values finite."""
+    f = np.float32
+
+    def one(x, bits, top, r16):
+        n = x.size
+        rows = np.append(x, np.zeros(-n % BLOCK, f)).astype(f).reshape(-1, BLOCK)
+        amax = rows.max(1)
+        s = np.where(amax < f(2.0 ** -100), f(0), amax * f(1 / 1.875)).astype(f)
+        with np.errstate(divide="ignore"):
+            inv = np.where(s > 0, f(1) / s, f(0)).astype(f)
+        t = (rows * inv[:, None]).reshape(-1)[:n]
+        u = (t * f(2.0 ** -112)).astype(f).view(np.uint32).astype(np.uint64)
+        drop = np.uint64(23 - bits)
+        c = (u + (r16.astype(np.uint64) << np.uint64(7 - bits))) >> drop
+        return np.minimum(c, top), s, t >= 2.0 ** -14
+
+    cm, sm, am = one(np.abs(m), 3, 127, r & np.uint64(0xFFFF))
+    root = np.sqrt(v)
+    cv, sv, av = one(root, 4, 254, r >> np.uint64(16))
+    cm = np.where((m < 0) & (cm > 0), cm + 128, cm)
+    cv = np.where(root > 0, np.maximum(cv, 1), 0)
+    return cm.astype(np.uint8), sm, cv.astype(np.uint8), sv, am & av
 
 
 # ---- the norm ------------------------------------------------------------------------------------------

@@ -219,6 +219,51 @@ def test_moments_seeds(gpu, seed, t):
     s.compare(before, s.state(), lr=1e-3, t=t, seed=seed)
 
 
+@pytest.mark.parametrize("seed", [0, 1234567])
+@pytest.mark.parametrize("size", [2.0 ** -30, 1.0, 2.0 ** 10])
+def test_bytes_are_those_of_fp32(gpu, size, seed):
+    """The bytes and scales are those of the documented fp32 operations, exactly (in the gradual
+    underflow, below 2^-14 of a block's largest, the order of two products is open: see check_codes)."""
+    s = Setup(gpu, [70001, 300, 256], eight=True, seed=18)
+    for v in s.g.views:
+        v.mul_(size)
+    for t in (1, 2, 3):
+        a = s.state()
+        s.plan.step_(lr=1e-3, step=t, grad_scale=0.5, seed=seed)
+        b = s.state()
+        for i, n in enumerate(s.sizes):
+            # the old values: one product for m, one and its square for v
+            m0 = R.values8(a[i]["mc"], a[i]["ms"], 3).astype(np.float32)
+            r0 = R.values8(a[i]["vc"], a[i]["vs"], 4).astype(np.float32)
+            _, m, v = R.step32(a[i]["p"], a[i]["g"], m0, r0 * r0, lr=1e-3, t=t, mult=0.5)
+            r = R.random_words(seed, t, i, np.arange(n)) if seed else np.full(n, 0x80008000, np.uint64)
+            cm, sm, cv, sv, above = R.encode32(m, v, r)
+            assert np.array_equal(sm, b[i]["ms"]) and np.array_equal(sv, b[i]["vs"]), (t, i)
+            assert np.array_equal(cm[above], b[i]["mc"][above]) and np.array_equal(cv[above], b[i]["vc"][above]), (t, i)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-16, 1e-8, 1e20])
+@pytest.mark.parametrize("size", [1e-18, 1e-12, 1e-7, 1e6, 1e17])
+def test_moments_of_every_size(gpu, size, eps):
+    """8-bit moments whose blocks lie outside the short path in one way or another: tiny and huge
+    gradients, every kind of eps, blocks with nothing in them beside others."""
+    s = Setup(gpu, [256 * 5 + 40, 3], "f32", False, "f32", True, seed=19, eps=eps, wd=[0.1, 0.0])
+    g = s.g.views[0]
+    g.mul_(size)
+    g[256:512] = 0.0
+    for x in (s.m.views[0], s.v.views[0]):
+        x[256:512] = 0
+        x[700:720] = 0
+    g[700:720] = size  # so that no quotient is 0 / 0 with eps 0 there
+    if eps == 0.0:
+        g[256:512] = size * 1e-3
+    for t in (1, 2):
+        before = s.state()
+        s.plan.step_(lr=1e-3, step=t, seed=77)
+        s.compare(before, s.state(), lr=1e-3, t=t, seed=77)
+    s.guards()
+
+
 def test_stochastic_rounding_keeps_the_mean(gpu):
     """v drifting by 0.1 % a step: rounded to nearest it stands still, by the seed its mean follows.
     The largest element holds its block's scale, so the others' bytes have to move by themselves."""
@@ -431,6 +476,72 @@ def test_two_graphs_of_one_plan(gpu):
         b.plan.grad_norm_(cb, max_norm=(0.1, 0.01)[k % 2])
         b.plan.step_(ctrl=cb)
         assert torch.equal(a.p.buf, b.p.buf) and torch.equal(ca.buffer, cb.buffer)
+
+
+def test_graph_of_a_bucket(gpu):
+    """A captured step that names its bucket: checked at the capture, replayed without the host."""
+    import torch
+
+    a, b = (Setup(gpu, RAGGED, grad="bf16", seed=33, bucket=True) for _ in range(2))
+    other = a.g.buf.clone()
+    ca, cb = (optim.Control(gpu, lr=1e-3) for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.plan.grad_norm_(ca, max_norm=0.1, bucket=other)
+        a.plan.step_(ctrl=ca, bucket=other)
+    for k in range(3):
+        other.mul_(-0.5)
+        graph.replay()
+        b.plan.grad_norm_(cb, max_norm=0.1, bucket=other)
+        b.plan.step_(ctrl=cb, bucket=other)
+        torch.cuda.synchronize()
+        assert torch.equal(a.p.buf, b.p.buf) and torch.equal(ca.buffer, cb.buffer), k
+
+
+def test_thousands_of_tensors(gpu):
+    """A long list of tiny tensors: one launch, every tensor with its own decay and rate."""
+    s = Setup(gpu, [1 + i % 37 for i in range(5000)], "f32", False, "f32", False, seed=3, pad=1)
+    before = s.state()
+    ctrl = optim.Control(gpu, lr=1e-3)
+    s.plan.grad_norm_(ctrl)
+    s.plan.step_(ctrl=ctrl)
+    norm, _ = R.norm64([x["g"] for x in before], 1.0, 0.0)
+    assert abs(ctrl.norm.item() - norm) <= 2 * R.U32 * norm
+    s.compare(before, s.state(), lr=float(np.float32(1e-3)), t=1)
+    s.guards()
+
+
+def test_threads_share_a_plan(gpu):
+    """Two threads, each with its stream, its ctrl and its bucket, over one plan of gradients."""
+    import threading
+
+    import torch
+
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(1)
+    bucket = torch.randn(200000, generator=gen, device=gpu)
+    plan = optim.AdamW(None, [bucket[:70000], bucket[70001:200000]], bucket=bucket)
+    others = [torch.randn(200000, generator=gen, device=gpu) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        side = torch.cuda.Stream()
+        ctrl = optim.Control(gpu)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(50):
+                plan.grad_norm_(ctrl, bucket=others[i])
+        side.synchronize()
+        got[i] = (ctrl.norm.item(), ctrl.step.item())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for i in range(2):
+        x = f64(others[i])
+        norm, _ = R.norm64([x[:70000], x[70001:200000]], 1.0, 0.0)
+        assert got[i][1] == 50 and abs(got[i][0] - norm) <= 2 * R.U32 * norm
 
 
 def test_other_stream(gpu):

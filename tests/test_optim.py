@@ -221,3 +221,16 @@ def test_reference_check_sees_wrong_bytes():
     codes[7] ^= 1
     with pytest.raises(AssertionError):
         R.check_codes(x, np.abs(x) * R.U32, codes, np.array([s]), 3, np.full(256, 0.5))
+
+
+def test_reference_fp32_bytes_are_the_definitions():
+    """encode32, the fp32 form operation by operation, passes check_codes, the definition in 64 bits."""
+    rng = np.random.default_rng(4)
+    n = 256 * 40 + 17
+    m = (rng.normal(0, 1, n) * 2.0 ** rng.integers(-12, 3, n)).astype(np.float32)
+    v = ((rng.normal(0, 1, n) * 2.0 ** rng.integers(-12, 3, n)) ** 2).astype(np.float32)
+    for r in (R.random_words(9, 4, 2, np.arange(n)), np.full(n, 0x80008000, np.uint64)):
+        cm, sm, cv, sv, _ = R.encode32(m, v, r)
+        R.check_codes(m.astype(np.float64), np.zeros(n), cm, sm, 3, (r & np.uint64(0xFFFF)) / 65536.0)
+        root = np.sqrt(v.astype(np.float64))
+        R.check_codes(root, R.U32 * root, cv, sv, 4, (r >> np.uint64(16)) / 65536.0)

@@ -2,9 +2,15 @@
 // (include/hydra_optim.h: the formulas and the 8-bit format).
 //
 // Every kernel here is a stream over HBM: AdamW moves 28 B per element with fp32 moments and 16
-// with 8-bit ones, the norm 4 or 2, the moment conversions 10 to 14.  No reuse, no MFMA.
-// A plan's tensors are cut into tiles; a workgroup finds its tile's tensor through a table with
-// one entry per tile, so one launch serves any number of tensors.
+// with 8-bit ones, the norm 4 or 2, the conversions of both moments 10 (from fp32) and 6 (to bf16).
+// No reuse, no MFMA; what bounds them is the rate at which HBM takes mixed reads and writes (a copy
+// 6.3 TB/s, reads alone 6.8), and for 8-bit moments nearly the vector units too (60 issue slots per
+// element, 103 us for 64 Mi elements if nothing else ran).
+// A plan's tensors are cut into tiles of 1024 elements, one workgroup each (64 Mi fp32: 4096 elements
+// by a loop took 346 us where one turn took 320).  A workgroup finds its tile's tensor through a table
+// with one entry per tile, so one launch serves any number of tensors; a single tensor's descriptor
+// passed in the launch itself was no faster.
+// Times below are of whole calls in sequence on rotating buffers, us, unless a kernel is named.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -70,8 +76,8 @@ typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t w2b __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t w1 __attribute__((aligned(1)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-// Nontemporal both ways: a step's state is larger than the caches.  64 Mi fp32: 344 us, against 368
-// with plain stores, 362 with plain loads and 361 with both plain.
+// Nontemporal both ways: a step's state is larger than the caches.  64 Mi fp32 322, plain loads 350,
+// plain stores 347; with 8-bit moments 235, 257 and 271.
 template <typename V>
 __device__ __forceinline__ V ldv(gptr p, uint32_t off) {
   return __builtin_nontemporal_load((const GLOBAL V*)(p + off));
@@ -177,7 +183,7 @@ __device__ __forceinline__ uint32_t load_bytes(gptr p, uint32_t i, uint32_t coun
   return w;
 }
 __device__ __forceinline__ void store_bytes(gptr p, uint32_t i, uint32_t w, uint32_t count) {
-  if (count >= 4) {  // not nontemporal: 4 bytes per lane are joined in the cache (178 -> 170 us)
+  if (count >= 4) {  // not nontemporal: 4 bytes per lane join in the cache (64 Mi both ways 175, else 186)
     *(GLOBAL w1*)(p + i) = w;
     return;
   }
@@ -231,7 +237,11 @@ __device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, 
   p = weight(p, m, v, k);
 }
 
-// fp32 moments: a workgroup takes one tile, 4 elements per lane.
+// fp32 moments: a workgroup takes one tile, 4 elements per lane.  Tiles in launch order: dealing each
+// XCD a contiguous eighth took 1287 instead of 1265 (256 Mi, bf16 with master) and 136 instead of 124
+// (291 ragged tensors, clipped), though 312 instead of 322 for one 64 Mi buffer.  The kernel alone:
+// 298 us for 64 Mi fp32 (6.3 TB/s), 1241 for the 256 Mi (6.06), 104 for the ragged tensors' 624 MB.
+// fp32 square root and quotient are IEEE's: replacing both by the hardware's estimates gained nothing.
 template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
                                                      const uint32_t* tile_tensor, OptStep st,
@@ -286,7 +296,10 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
 }
 
 // 8-bit moments: a workgroup takes one tile, a wave one block of 256 elements of it, 4 per lane, so a
-// block's scales are wave-uniform.
+// block's scales are wave-uniform.  The kernel alone: 164 us for 64 Mi fp32 (1078 MB, 6.6 TB/s: some of
+// the bytes of the last call are still in the Infinity Cache), 231 for 397 tensors of 100 M elements in
+// bf16 with master.  Each XCD a contiguous eighth of the tiles: 235 with what follows it, in launch
+// order 239; the ragged tensors 371 and 386.
 static_assert(kOptTile == kOptBlock * 4 && kOptTile == kOptBlock / 64 * kMomentBlock, "one turn");
 // lanes 31 and 63: the largest of their half of the wave
 __device__ __forceinline__ uint32_t half_wave_umax(uint32_t x) {
@@ -319,18 +332,18 @@ __device__ __forceinline__ uint32_t add_high16(uint32_t c, uint32_t r) {
 // The square root of v >= 0, not denormal, rounded as sqrtf rounds it, in 8 issue slots instead of 17:
 // the reciprocal root's estimate s, then s + (v - s^2) / (2 s) (all 2^24 values of [1, 4) checked
 // against sqrtf; below 2^-98 the rest v - s^2 itself is rounded, and 1 ulp may be off).  A denormal
-// becomes something below 2^-63; what is not finite, something not finite.
+// becomes something above 0 and below 2^-62; what is not finite, something not finite.
 __device__ __forceinline__ float plain_sqrt(float v) {
   const float r = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f));
   const float s = v * r;
   return fmaf(fmaf(-s, s, v), 0.5f * r, s);
 }
 // What a block's largest magnitude (its bits) has to be for the encoders below: 2^-112 / scale is
-// normal, and every value is finite.  sqrt v also not below 2^-44: what plain_sqrt does not see in
+// normal, and every value is finite.  sqrt v also 0, or not below 2^-43: what plain_sqrt makes of
 // denormals lies under the smallest byte then.
 __device__ __forceinline__ bool plain_m(uint32_t top) { return top < fbits(0x1p14f); }
 __device__ __forceinline__ bool plain_root(uint32_t top) {
-  return top - fbits(0x1p-44f) < fbits(0x1p14f) - fbits(0x1p-44f);
+  return top == 0 || top - fbits(0x1p-43f) < fbits(0x1p14f) - fbits(0x1p-43f);
 }
 // 2^-112 / scale (0 for an empty block)
 __device__ __forceinline__ float plain_inv(float scale) { return moment_inv(scale) * 0x1p-112f; }
@@ -361,7 +374,9 @@ __device__ __forceinline__ float uniform(float x, int lane) {
   return bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(x), lane));
 }
 
-// A block's four elements per lane: decode, step, encode.  The bytes are those of the documented
+// A block's four elements per lane: decode, step, encode.  The vector units have 91 issue slots per
+// element while HBM delivers its 16 bytes; this takes 60 (counted in the assembly; with an IEEE
+// quotient in p's update the kernel took 170 us instead of 164).  The bytes are those of the documented
 // operations, each rounded to fp32.  Decoding is short where no byte stands for something not finite
 // and both old scales are below 2^15 (2^112 * scale is finite: one product per value).  The rest is
 // short where the block is plain (above) and eps lies in [2^-40, 2^60]: eps hides what plain_sqrt
@@ -498,9 +513,10 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
 // ---- the norm --------------------------------------------------------------------------------------
 // fp64 sums: no gradient's square overflows, and the sum is not finite exactly when some gradient
 // is not.  The order is the grid's, which the plan fixes: workgroup b sums a contiguous run of tiles,
-// and one workgroup adds the sums -- in a launch of its own: counting arrivals at one address instead
-// took 10 ns for each workgroup, 36 with the cache's write-back, and 4.5 us in all is the launch.
-// A plan of at most kNormAlone tiles is one workgroup's, in one launch.
+// and one workgroup adds the sums in a second launch (4.5 us, nearly all of it the launch; the
+// workgroups counting their arrivals in the first one instead cost 9 us more for 1024 of them, 36
+// where the count also writes the caches back).  A plan of at most kNormAlone tiles is one
+// workgroup's, in one launch (4 Ki fp32: 3.5 us, against 2.8 + 4.5).
 constexpr int kNormAloneBlock = 1024;
 constexpr uint32_t kNormAlone = 32;
 
@@ -558,9 +574,11 @@ __device__ __forceinline__ w4 vector_or_zero(gptr at, uint64_t left) {
   return x;
 }
 
+// 2048 workgroups, 32 waves per CU: 64 Mi fp32 42 us (6.4 TB/s), 397 bf16 tensors of 100 M elements
+// 34 (5.9); fp32 sums instead of fp64 were no faster.
 // ALONE: the only workgroup, which finishes too.  KEEP: leave the gradients in the caches for the step
 // that reads them next: the norm alone takes 10 % longer, the two together 5 to 10 % less (128 MiB of
-// fp32 gradients 181 -> 162 us, 512 MiB 724 -> 700).  A plan of gradients alone has no step.
+// fp32 gradients 181 -> 162 us, 512 MiB 724 -> 702).  A plan of gradients alone has no step.
 template <typename G, int BS, bool ALONE, bool KEEP>
 __global__ __launch_bounds__(BS) void k_norm(const OptTensor* tensors, const uint32_t* tile_tensor,
                                              uint32_t each, uint32_t more, uint64_t bucket,
@@ -638,7 +656,7 @@ __device__ __forceinline__ uint32_t wave_part(size_t n, size_t* at) {
 }
 
 // encode: 4 elements per lane of each block, all loads first (8 consecutive ones per lane leave every
-// fp32 load half of the lines it touches)
+// fp32 load half of the lines it touches: 127 us for 64 Mi, this 112, 6.0 TB/s)
 template <typename E>
 __global__ __launch_bounds__(kOptBlock) void k_encode(uint8_t* m8, float* ms, uint8_t* v8,
                                                       float* vs, const E* m, const E* v, size_t n) {
@@ -705,7 +723,8 @@ __global__ __launch_bounds__(kOptBlock) void k_encode(uint8_t* m8, float* ms, ui
   }
 }
 
-// decode: 8 consecutive elements per lane
+// decode: 8 consecutive elements per lane, so a bf16 store is 16 bytes (64 Mi: 66 us, 6.1 TB/s; 4 per
+// lane 84)
 struct Part {
   uint32_t i, count, lo, hi;  // the lane's first element; how many it has, in all and by fours
 };

@@ -161,7 +161,8 @@ class AdamW:
         cfg = _lib.AdamWConfig(0 if norm_only else _code(lists["params"][0].dtype),
                                _code(self._grad_dtype),
                                _lib.UINT8 if eight else _lib.FLOAT32, flags, betas[0], betas[1], eps)
-        L = _lib.lib()
+        self._bucket_at = base if bucket is not None else None
+        L = self._L = _lib.lib()
         check(L.hydra_adamw_create(self._index, ctypes.byref(cfg), table.ctypes.data, k,
                                    ctypes.byref(self._h)))
         size = ctypes.c_size_t()
@@ -176,26 +177,23 @@ class AdamW:
 
     def _bucket_ptr(self, bucket):
         if self._bucket is None:
-            if bucket is not None:
-                _refuse("AdamW: the plan was made without a bucket")
-            return None
+            _refuse("AdamW: the plan was made without a bucket")
         if bucket is None:
-            return self._bucket.data_ptr()
+            return self._bucket_at
         self._check_bucket_tensor(bucket, self._bucket)
         if bucket.numel() * bucket.element_size() < self._bucket_bytes:
             _refuse("AdamW: the bucket is shorter than the plan's")
         return bucket.data_ptr()
 
-    def _handle(self):
-        if not self._h:
-            _refuse("AdamW: the plan is closed")
-        return self._h
+    def _closed(self):
+        _refuse("AdamW: the plan is closed")
 
     def grad_norm_(self, ctrl: Control, max_norm: float = 0.0, grad_scale: float = 1.0, bucket=None,
                    stream: int | None = None) -> None:
         """hydra_adamw_grad_norm: norm, clip factor and finite check of all gradients into ctrl, and
         the next step's number.  max_norm 0: no clipping."""
-        h, b = self._handle(), self._bucket_ptr(bucket)
+        h = self._h or self._closed()
+        b = self._bucket_ptr(bucket) if self._bucket is not bucket else self._bucket_at
         if ctrl.index != self._index:
             _refuse("grad_norm_: ctrl is on another device")
         s, ws, size = stream, None, self._workspace
@@ -206,25 +204,28 @@ class AdamW:
             if stream is not None and stream != _current_stream(self._index):
                 ws.record_stream(torch.cuda.ExternalStream(stream, device=self.device))
             ws = ws.data_ptr()
-        check(_lib.lib().hydra_adamw_grad_norm(h, b, grad_scale, max_norm, ctrl.ptr, ws, size, s))
+        check(self._L.hydra_adamw_grad_norm(h, b, grad_scale, max_norm, ctrl.ptr, ws, size, s))
 
     def step_(self, lr: float | None = None, step: int | None = None, grad_scale: float = 1.0,
               ctrl: Control | None = None, seed: int = 0, bucket=None,
               stream: int | None = None) -> None:
         """One AdamW step in place: with lr and step (1, 2, ...) from the arguments, or with ctrl
         from the last grad_norm_ on it.  seed: that of the 8-bit moments' rounding (0: to nearest)."""
-        h, b = self._handle(), self._bucket_ptr(bucket)
-        s = stream if stream is not None else _current_stream(self._index)
+        h = self._h or self._closed()
+        b = self._bucket_ptr(bucket) if self._bucket is not bucket else self._bucket_at
+        s = _current_stream(self._index) if stream is None else stream
         if ctrl is not None:
             if lr is not None or step is not None or grad_scale != 1.0:
                 _refuse("step_: lr, step and grad_scale come from ctrl")
             if ctrl.index != self._index:
                 _refuse("step_: ctrl is on another device")
-            check(_lib.lib().hydra_adamw_step_ctrl(h, b, ctrl.ptr, seed, s))
-            return
-        if lr is None or step is None:
-            _refuse("step_: lr and step, or ctrl")
-        check(_lib.lib().hydra_adamw_step(h, b, lr, step, grad_scale, seed, s))
+            rc = self._L.hydra_adamw_step_ctrl(h, b, ctrl.ptr, seed, s)
+        else:
+            if lr is None or step is None:
+                _refuse("step_: lr and step, or ctrl")
+            rc = self._L.hydra_adamw_step(h, b, lr, step, grad_scale, seed, s)
+        if rc:
+            check(rc)
 
     def close(self) -> None:
         """Waits for the device's work, then releases the plan."""
@@ -251,37 +252,45 @@ def _moments(m, v, m8, m_scale, v8, v_scale):
     n, dtype, index = some.numel(), some.dtype, some.get_device()
     if index < 0:
         _refuse("moments8: contiguous tensors on one GPU are required")
-    pointers = []
-    for x, codes, scale, name in ((m, m8, m_scale, "m"), (v, v8, v_scale, "v")):
+    rows = -(-n // MOMENT_BLOCK)
+
+    def pointers(x, codes, scale, name):
         if x is None:
             if codes is not None or scale is not None:
                 _refuse(f"moments8: codes or scales of {name} without its values")
-            pointers.append((None, None, None))
-            continue
+            return None, None, None
         if codes is None or scale is None:
             _refuse(f"moments8: {name} needs its codes and its scales")
-        for t in (x, codes, scale):
-            if t.get_device() != index or not t.is_contiguous():
-                _refuse("moments8: contiguous tensors on one GPU are required")
-        if codes.dtype != torch.uint8 or scale.dtype != torch.float32 or x.dtype != dtype:
+        if not (x.get_device() == codes.get_device() == scale.get_device() == index
+                and x.is_contiguous() and codes.is_contiguous() and scale.is_contiguous()):
+            _refuse("moments8: contiguous tensors on one GPU are required")
+        if codes.dtype is not torch.uint8 or scale.dtype is not torch.float32 or x.dtype is not dtype:
             _refuse("moments8: uint8 codes, float32 scales and values of one dtype are required")
-        if x.numel() != n or codes.numel() != n or scale.numel() != moment_scales(n):
+        if x.numel() != n or codes.numel() != n or scale.numel() != rows:
             _refuse(f"moments8: {name}: lengths do not fit {n} elements")
-        pointers.append((x.data_ptr(), codes.data_ptr(), scale.data_ptr()))
-    return index, _code(dtype), n, *pointers
+        return x.data_ptr(), codes.data_ptr(), scale.data_ptr()
+
+    return index, _code(dtype), n, pointers(m, m8, m_scale, "m"), pointers(v, v8, v_scale, "v")
+
+
+def _on(index: int, call, *args) -> None:
+    """A C call that works on the current device, made on device `index`."""
+    if torch.cuda.current_device() == index:
+        check(call(*args))
+    else:
+        with torch.cuda.device(index):
+            check(call(*args))
 
 
 def moments8_encode_(m8, m_scale, v8, v_scale, m, v, stream: int | None = None) -> None:
     """One tensor's moments (fp32 or bf16) into 8 bits, to nearest; either moment may be None."""
     index, code, n, pm, pv = _moments(m, v, m8, m_scale, v8, v_scale)
-    with torch.cuda.device(index):
-        s = stream if stream is not None else _current_stream(index)
-        check(_lib.lib().hydra_moments8_encode(pm[1], pm[2], pv[1], pv[2], pm[0], pv[0], code, n, s))
+    s = _current_stream(index) if stream is None else stream
+    _on(index, _lib.lib().hydra_moments8_encode, pm[1], pm[2], pv[1], pv[2], pm[0], pv[0], code, n, s)
 
 
 def moments8_decode_(m, v, m8, m_scale, v8, v_scale, stream: int | None = None) -> None:
     """The values that 8-bit moments stand for, into fp32 or bf16; either moment may be None."""
     index, code, n, pm, pv = _moments(m, v, m8, m_scale, v8, v_scale)
-    with torch.cuda.device(index):
-        s = stream if stream is not None else _current_stream(index)
-        check(_lib.lib().hydra_moments8_decode(pm[0], pv[0], code, pm[1], pm[2], pv[1], pv[2], n, s))
+    s = _current_stream(index) if stream is None else stream
+    _on(index, _lib.lib().hydra_moments8_decode, pm[0], pv[0], code, pm[1], pm[2], pv[1], pv[2], n, s)

@@ -29,13 +29,15 @@ extern "C" {
  * `param` without a master loses updates below half a step of its type.
  *
  * 8-bit moments (state_dtype HYDRA_UINT8): each 256 consecutive elements of a tensor share one
- * fp32 scale per moment, s = (their largest finite magnitude) / 1.875; a block whose magnitudes
- * all lie below 2^-100 is stored as zeros.
+ * fp32 scale per moment, s = (their largest finite magnitude) * fp32(1 / 1.875); a block whose
+ * magnitudes all lie below 2^-100 has scale 0 and reads as zeros.
  *     m        byte = sign << 7 | c;  value = +-F3(c) * s;  byte 0x80: not finite, reads as NaN
  *     sqrt(v)  byte = c;              value = F4(c) * s, v = value^2;  255: not finite, reads as inf
  * with Fk the float of 4 exponent bits and k mantissa bits whose largest power of two is 1:
  * Fk(c) = c * 2^-(14 + k) for c < 2^k, else 2^((c >> k) - 15) * (1 + (c mod 2^k) / 2^k).  A v above
- * zero never becomes zero (its byte is at least 1), so no step divides by eps alone.
+ * zero never becomes zero (its byte is at least 1), so no step divides by eps alone.  m, v and the
+ * bytes come from the operations above, each rounded to fp32 (x = |value| * (1 / s)); the quotient in
+ * p's update is within 2 units in the last place.
  * A step rounds its new moments stochastically: with x the magnitude over s, the two bytes around
  * x are taken with probabilities that make the mean x, by 16 random bits for each moment from a
  * 32-bit hash of (seed, t, the tensor's place in the plan, i) -- the same bits on every run and

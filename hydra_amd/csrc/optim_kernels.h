@@ -12,12 +12,13 @@ namespace hydra {
 constexpr int kOptBlock = 256;      // 4 waves of 64 lanes
 constexpr int kMomentBlock = 256;   // elements that share one scale of an 8-bit moment
 constexpr size_t kOptTile = 1024;   // elements of one tensor that a workgroup takes
+constexpr uint32_t kMaxHead = 64;   // a head is one element per lane of one wave at most
 constexpr int kNormBlocks = 2048;   // workgroups (and partial sums) of the norm, at most
 
 // One tensor of a plan, in device memory.  `grad` counts from the bucket that a call gives (null:
 // an address).  Its tile k is number tile0 + k and holds the elements [head + k * kOptTile,
-// head + (k + 1) * kOptTile), the first one those before them too: `head` (0 to 3) puts the vectors
-// of as many of its buffers as possible on their natural alignment.
+// head + (k + 1) * kOptTile), the first one those before them too: `head` puts the vectors of as many
+// of its buffers as possible on their natural alignment, and their tiles on whole lines.
 struct OptTensor {
   char* param;
   float* master;

@@ -238,9 +238,9 @@ __device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, 
 }
 
 // fp32 moments: a workgroup takes one tile, 4 elements per lane.  Tiles in launch order: dealing each
-// XCD a contiguous eighth took 1287 instead of 1265 (256 Mi, bf16 with master) and 136 instead of 124
-// (291 ragged tensors, clipped), though 312 instead of 322 for one 64 Mi buffer.  The kernel alone:
-// 298 us for 64 Mi fp32 (6.3 TB/s), 1241 for the 256 Mi (6.06), 104 for the ragged tensors' 624 MB.
+// XCD a contiguous eighth took 1287 instead of 1265 (256 Mi, bf16 with master), though 312 instead of
+// 322 for one 64 Mi buffer.  The kernel alone: 296 us for 64 Mi fp32 (6.35 TB/s), 1240 for the 256 Mi
+// (6.06), 95 for 291 ragged tensors' 624 MB.
 // fp32 square root and quotient are IEEE's: replacing both by the hardware's estimates gained nothing.
 template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
@@ -275,8 +275,9 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
     At<float>::store4(mm, i, a);
     At<float>::store4(vv, i, b);
   }
-  // the tensor's ragged ends, one element per lane: up to 3 before the first tile's vectors (wave 0)
-  // and up to 3 after the last one's (wave 1)
+  // the tensor's ragged ends, one element per lane: those before the first tile's vectors (wave 0) and
+  // up to 3 after the last one's (wave 1)
+  static_assert(kMaxHead <= 64, "one wave takes the head");
   const uint32_t before = tile == T.tile0 ? T.head : 0u, after = left & 3;
   if (before | after) {
     const uint32_t t = threadIdx.x;

@@ -35,6 +35,7 @@ _CODES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.floa
 # the current stream's handle by device index (torch.cuda.current_stream builds a Stream object
 # around it: 2 us, as long as a small step's kernel runs)
 _current_stream = torch._C._cuda_getCurrentRawStream
+_left = []  # handles of plans dropped during a capture: released when the next plan is made
 
 
 def moment_scales(n: int) -> int:
@@ -84,12 +85,15 @@ class AdamW:
     writes.  weight_decay and lr_scale: a number, or one for each tensor.  params None: a plan for
     grad_norm_ alone.  bucket: a 1-d tensor whose views the grads are; each call may then name
     another bucket of that layout (two buckets in turn, one being reduced while the other is
-    stepped).  The plan keeps the tensors alive; a graph that holds its calls does not."""
+    stepped).  The plan keeps the tensors alive; a graph that holds its calls does not.  Calls write
+    the tensors past autograd: nothing that a backward pass still needs may be among them."""
 
     def __init__(self, params, grads, m=None, v=None, *, master=None, m_scale=None, v_scale=None,
                  betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0,
                  bucket=None):
         self._h = ctypes.c_void_p()
+        while _left and not torch.cuda.is_current_stream_capturing():
+            _lib.lib().hydra_adamw_destroy(_left.pop())
         grads = _list(grads)
         if not grads:
             _refuse("AdamW: no tensors")
@@ -228,7 +232,7 @@ class AdamW:
             check(rc)
 
     def close(self) -> None:
-        """Waits for the device's work, then releases the plan."""
+        """Waits for the device's work, then releases the plan (not while a stream is captured)."""
         if self._h:
             _lib.lib().hydra_adamw_destroy(self._h)
             self._h = ctypes.c_void_p()
@@ -239,6 +243,9 @@ class AdamW:
         if _is_finalizing is None or _is_finalizing():
             return
         try:
+            if self._h and torch.cuda.is_current_stream_capturing():
+                _left.append(self._h)  # waiting for the device would end the capture
+                return
             self.close()
         except Exception:
             pass

@@ -434,9 +434,14 @@ def test_graph_replays(gpu):
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         graph = torch.cuda.CUDAGraph()
+        values = torch.empty(4097, device=gpu)
+        dropped = [Setup(gpu, [10])]
         with torch.cuda.graph(graph, stream=side):
             a.plan.grad_norm_(ca, max_norm=0.1)
+            dropped.clear()  # a plan that goes during a capture does not end it
             a.plan.step_(ctrl=ca, seed=4)
+            if eight:
+                optim.moments8_decode_(values, None, a.m.views[0], a.ms.views[0], None, None)
         gen = torch.Generator(device=gpu)
         for k in range(6):
             gen.manual_seed(k)
@@ -455,6 +460,9 @@ def test_graph_replays(gpu):
             for x, y in ((a.p, b.p), (a.pm, b.pm), (a.m, b.m), (a.v, b.v)):
                 assert torch.equal(x.buf, y.buf), k
             assert torch.equal(ca.buffer, cb.buffer), k
+            if eight:
+                want = R.values8(b.m.views[0].cpu().numpy(), b.ms.views[0].cpu().numpy(), 3)
+                assert (np.abs(f64(values) - want) <= R.U32 * np.abs(want)).all(), k
         assert ca.step.item() == 5 and ca.skipped.item() == 1
         del graph
 

@@ -18,12 +18,13 @@ extern "C" {
 
 /* ---- the tensors of a step ------------------------------------------------------------------
  * A plan is the list of tensors a training program steps together, laid out once on the device.
- * Per element i of a tensor, with t the number of the step (1, 2, ...), lr' = lr * lr_scale and
+ * Per element i of a tensor, with t the number of the step (1, 2, ...), lr' = lr * lr_scale,
+ * c1 = 1 / (1 - beta1^t) and c2 = 1 / sqrt(1 - beta2^t) (those and 1 - beta in fp64, rounded once) and
  * every operation rounded to fp32 in the order written:
  *     g = float(grad[i]) * mult
  *     m = m * beta1 + g * (1 - beta1)
  *     v = v * beta2 + (g * (1 - beta2)) * g
- *     p = p * (1 - lr' * weight_decay) - (m / (sqrt(v) / sqrt(1 - beta2^t) + eps)) * (lr' / (1 - beta1^t))
+ *     p = p * (1 - lr' * weight_decay) - (m / (sqrt(v) * c2 + eps)) * (lr' * c1)
  * p is the fp32 master where there is one (`param` is then written only: the master rounded to
  * nearest even), else `param` widened, and rounded to nearest even on its way back.  A 16-bit
  * `param` without a master loses updates below half a step of its type.
@@ -34,10 +35,10 @@ extern "C" {
  *     m        byte = sign << 7 | c;  value = +-F3(c) * s;  byte 0x80: not finite, reads as NaN
  *     sqrt(v)  byte = c;              value = F4(c) * s, v = value^2;  255: not finite, reads as inf
  * with Fk the float of 4 exponent bits and k mantissa bits whose largest power of two is 1:
- * Fk(c) = c * 2^-(14 + k) for c < 2^k, else 2^((c >> k) - 15) * (1 + (c mod 2^k) / 2^k).  A v above
- * zero never becomes zero (its byte is at least 1), so no step divides by eps alone.  m, v and the
- * bytes come from the operations above, each rounded to fp32 (x = |value| * (1 / s)); the quotient in
- * p's update is within 2 units in the last place.
+ * Fk(c) = c * 2^-(14 + k) for c < 2^k, else 2^((c >> k) - 15) * (1 + (c mod 2^k) / 2^k).  The byte
+ * of a v above zero is at least 1, so no step divides by eps alone where fp32 holds v at all.  m, v
+ * and the bytes come from the operations above, each rounded to fp32 (x = |value| * (1 / s)); the
+ * quotient in p's update is within 2 units in the last place.
  * A step rounds its new moments stochastically: with x the magnitude over s, the two bytes around
  * x are taken with probabilities that make the mean x, by 16 random bits for each moment from a
  * 32-bit hash of (seed, t, the tensor's place in the plan, i) -- the same bits on every run and

@@ -225,6 +225,7 @@ int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_ten
     }
   }
   P.table.tiles = (uint32_t)tiles;
+  P.table.filled = (uint32_t)grads.size();
   if (tiles == 0) return HYDRA_OK;
 
   // [descriptors | the tensor of each tile], through a pinned block
@@ -384,7 +385,7 @@ int hydra_adamw_destroy(hydra_adamw_t plan) {
 
 int hydra_adamw_workspace(hydra_adamw_t plan, size_t* bytes) {
   if (!plan || !bytes) return fail(HYDRA_ERR_INVALID, "null plan or bytes");
-  *bytes = hydra::norm_workspace(plan->table.tiles);
+  *bytes = hydra::norm_workspace(plan->table);
   return ok();
 }
 
@@ -397,7 +398,7 @@ int hydra_adamw_grad_norm(hydra_adamw_t plan, const void* bucket, double grad_sc
   if (!(max_norm >= 0.0)) return fail(HYDRA_ERR_INVALID, "max_norm must be >= 0");
   if (!aligned(ctrl, 8) || !aligned(workspace, 8))
     return fail(HYDRA_ERR_INVALID, "ctrl and workspace must be 8-byte aligned");
-  const size_t need = hydra::norm_workspace(plan->table.tiles);
+  const size_t need = hydra::norm_workspace(plan->table);
   if (workspace_bytes < need || (need && !workspace))
     return fail(HYDRA_ERR_INVALID, "workspace smaller than hydra_adamw_workspace says");
   if (int rc = check_bucket(*plan, bucket)) return rc;

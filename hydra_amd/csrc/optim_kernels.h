@@ -38,6 +38,7 @@ struct OptTable {
   const OptTensor* tensors;      // device
   const uint32_t* tile_tensor;   // device: the tensor of each tile
   uint32_t tiles;
+  uint32_t filled;               // tensors that have elements
 };
 
 // A step's scalars: by value, or (ctrl) the device's.
@@ -73,7 +74,7 @@ __host__ __device__ inline double power(double beta, uint64_t t) {
 
 hipError_t launch_adamw(const hydra_adamw_config_t& cfg, const OptTable& t, const OptStep& step,
                         const void* bucket, hipStream_t s);
-size_t norm_workspace(uint32_t tiles);  // bytes of partial sums
+size_t norm_workspace(const OptTable& t);  // bytes of partial sums
 hipError_t launch_grad_norm(const hydra_adamw_config_t& cfg, const OptTable& t, const OptNorm& norm,
                             const void* bucket, hydra_adamw_ctrl_t* ctrl, double* partials,
                             hipStream_t s);

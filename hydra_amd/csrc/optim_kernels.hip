@@ -516,10 +516,11 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
 // is not.  The order is the grid's, which the plan fixes: workgroup b sums a contiguous run of tiles,
 // and one workgroup adds the sums in a second launch (4.5 us, nearly all of it the launch; the
 // workgroups counting their arrivals in the first one instead cost 9 us more for 1024 of them, 36
-// where the count also writes the caches back).  A plan of at most kNormAlone tiles is one
-// workgroup's, in one launch (4 Ki fp32: 3.5 us, against 2.8 + 4.5).
+// where the count also writes the caches back).  A small plan is one workgroup's, in one launch: that
+// takes 0.6 us for each tensor in turn and 0.05 for each tile (fp32; bf16 0.04), where two launches
+// take 6.9 (1 tensor of 4 tiles 3.8 us, of 64 5.9, of 96 7.4; 6 tensors of 4 tiles 6.1, 8 7.4).
 constexpr int kNormAloneBlock = 1024;
-constexpr uint32_t kNormAlone = 32;
+bool norm_alone(const OptTable& t) { return t.tiles + 12 * (uint64_t)t.filled <= 96; }
 
 template <int BS>
 __device__ __forceinline__ double block_sum(double x, double* lds) {
@@ -816,7 +817,7 @@ template <typename G, bool KEEP>
 hipError_t norm_t(const OptTable& t, const OptNorm& norm, const void* bucket,
                   hydra_adamw_ctrl_t* ctrl, double* partials, hipStream_t s) {
   const uint64_t at = reinterpret_cast<uint64_t>(bucket);
-  if (t.tiles <= kNormAlone) {
+  if (norm_alone(t)) {
     hipLaunchKernelGGL((k_norm<G, kNormAloneBlock, true, KEEP>), dim3(1), dim3(kNormAloneBlock), 0,
                        s, t.tensors, t.tile_tensor, t.tiles, 0u, at, partials, norm, ctrl);
     return hipGetLastError();
@@ -885,8 +886,8 @@ hipError_t launch_adamw(const hydra_adamw_config_t& cfg, const OptTable& t, cons
                                         : adamw_p<false>(cfg, t, st, bucket, s);
 }
 
-size_t norm_workspace(uint32_t tiles) {
-  return tiles <= kNormAlone ? 0 : std::min(tiles, (uint32_t)kNormBlocks) * sizeof(double);
+size_t norm_workspace(const OptTable& t) {
+  return norm_alone(t) ? 0 : std::min(t.tiles, (uint32_t)kNormBlocks) * sizeof(double);
 }
 
 hipError_t launch_grad_norm(const hydra_adamw_config_t& cfg, const OptTable& t, const OptNorm& norm,

@@ -347,7 +347,8 @@ def test_eps_zero_and_all_zero(gpu):
 
 # ---- the norm -------------------------------------------------------------------------------------
 @pytest.mark.parametrize("grad", GRADS)
-@pytest.mark.parametrize("sizes", [[1], [4096], [4097, 1, 0, 255], [1 << 20, 3, 5_000_001], RAGGED * 8])
+@pytest.mark.parametrize("sizes", [[1], [4096], [4097, 1, 0, 255], [84 * 1024], [85 * 1024], [70, 0, 500, 1025, 3, 2000],
+                                   [9] * 7 + [0], [9] * 8, [1 << 20, 3, 5_000_001], RAGGED * 8])
 def test_norm(gpu, grad, sizes):
     """Norm, clip factor, step number and corrections; the same bits every time."""
     import torch

@@ -886,6 +886,7 @@ hipError_t launch_adamw(const hydra_adamw_config_t& cfg, const OptTable& t, cons
                                         : adamw_p<false>(cfg, t, st, bucket, s);
 }
 
+static_assert(kNormBlocks * sizeof(double) <= HYDRA_ADAMW_WORKSPACE_MAX, "the bound callers may allocate by");
 size_t norm_workspace(const OptTable& t) {
   return norm_alone(t) ? 0 : std::min(t.tiles, (uint32_t)kNormBlocks) * sizeof(double);
 }

@@ -31,6 +31,7 @@ from ._lib import HydraError, check
 _is_finalizing = sys.is_finalizing
 
 MOMENT_BLOCK = 256  # elements that share one scale of an 8-bit moment
+_WORKSPACE = 16384  # HYDRA_ADAMW_WORKSPACE_MAX (include/hydra_optim.h)
 _CODES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
 # the current stream's handle by device index (torch.cuda.current_stream builds a Stream object
 # around it: 2 us, as long as a small step's kernel runs)
@@ -61,13 +62,17 @@ def _refuse(msg: str):
 class Control:
     """hydra_adamw_ctrl_t: 64 bytes on the device that carry a step's scalars from grad_norm_ to
     step_ without a host round trip.  Its fields are 0-d device tensors: lr and step are set by the
-    program (ctrl.lr.fill_(x)), the others are written by grad_norm_."""
+    program (ctrl.lr.fill_(x)), the others are written by grad_norm_.  Behind them lies grad_norm_'s
+    workspace: calls on one Control go to one stream or are ordered by events, whatever their plans,
+    and a graph that holds such calls needs its Control."""
 
     def __init__(self, device, lr: float = 0.0, step: int = 0):
-        self.buffer = torch.zeros(64, dtype=torch.uint8, device=device)
-        if not self.buffer.is_cuda:
+        memory = torch.zeros(64 + _WORKSPACE, dtype=torch.uint8, device=device)
+        if not memory.is_cuda:
             _refuse("Control: a GPU device is required")
+        self.buffer = memory[:64]
         self.index, self.ptr = self.buffer.get_device(), self.buffer.data_ptr()
+        self.workspace = self.ptr + 64
         f, i = self.buffer.view(torch.float32), self.buffer.view(torch.int32)
         self.step, self.skipped = self.buffer.view(torch.int64)[:2]
         self.lr, self.mult, self.norm = f[4], f[5], f[6]
@@ -171,7 +176,7 @@ class AdamW:
                                    ctypes.byref(self._h)))
         size = ctypes.c_size_t()
         check(L.hydra_adamw_workspace(self._h, ctypes.byref(size)))
-        self._workspace = size.value
+        self._workspace = size.value  # 0: the norm is one launch
 
     @staticmethod
     def _check_bucket_tensor(b, like):
@@ -200,15 +205,11 @@ class AdamW:
         b = self._bucket_ptr(bucket) if self._bucket is not bucket else self._bucket_at
         if ctrl.index != self._index:
             _refuse("grad_norm_: ctrl is on another device")
-        s, ws, size = stream, None, self._workspace
-        if stream is None:
-            s = _current_stream(self._index)
-        if size:  # from torch's allocator, for this call: two graphs of one plan share none
-            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            if stream is not None and stream != _current_stream(self._index):
-                ws.record_stream(torch.cuda.ExternalStream(stream, device=self.device))
-            ws = ws.data_ptr()
-        check(self._L.hydra_adamw_grad_norm(h, b, grad_scale, max_norm, ctrl.ptr, ws, size, s))
+        s = _current_stream(self._index) if stream is None else stream
+        # the workspace is the Control's: memory allocated here would belong to the current stream, whose
+        # queued work may still use it when another stream writes it
+        check(self._L.hydra_adamw_grad_norm(h, b, grad_scale, max_norm, ctrl.ptr, ctrl.workspace,
+                                            _WORKSPACE, s))
 
     def step_(self, lr: float | None = None, step: int | None = None, grad_scale: float = 1.0,
               ctrl: Control | None = None, seed: int = 0, bucket=None,

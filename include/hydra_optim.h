@@ -99,6 +99,8 @@ int hydra_adamw_create(int device, const hydra_adamw_config_t* config,
 /* Waits for the device's work, then releases the plan (not the tensors). */
 int hydra_adamw_destroy(hydra_adamw_t plan);
 
+#define HYDRA_ADAMW_WORKSPACE_MAX 16384 /* bytes: no plan needs a larger workspace */
+
 /* All calls below enqueue on `stream` of the plan's device whatever the caller's current device
  * is: asynchronous, no allocation, no synchronisation, graph-capturable.  They are ordered like
  * any in-place update: two calls on the same tensors (or the same ctrl or workspace) go to one
@@ -109,8 +111,10 @@ int hydra_adamw_destroy(hydra_adamw_t plan);
  * the same bits on every call and on every rank that holds the same bits.  max_norm > 0 clips:
  * mult = grad_scale * min(1, max_norm / (norm + 1e-6)); 0: mult = grad_scale.  If the sum is not
  * finite, skip = 1 and skipped += 1; else step += 1 and the fields for that step are set.
- * workspace: hydra_adamw_workspace() bytes of device memory (none for a small plan: NULL then),
- * 8-byte aligned, needed until the call has run; its contents do not matter. */
+ * workspace: hydra_adamw_workspace() bytes of device memory or more (none for a small plan: may be
+ * NULL then), 8-byte aligned, needed until the call has run, and by graphs that hold it; its contents
+ * do not matter.  It is written on `stream`: memory that another stream's work may still use has to be
+ * ordered first. */
 int hydra_adamw_workspace(hydra_adamw_t plan, size_t* bytes);
 int hydra_adamw_grad_norm(hydra_adamw_t plan, const void* bucket, double grad_scale,
                           double max_norm, hydra_adamw_ctrl_t* ctrl, void* workspace,

@@ -1,0 +1,82 @@
+"""How hydra_amd.optim makes its calls, without a GPU: plans whose library is a stand-in."""
+import ctypes
+import types
+
+import pytest
+
+from hydra_amd import optim
+
+torch = pytest.importorskip("torch")
+
+
+class Library:
+    """Takes every call and keeps its arguments."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+class Plan(optim.AdamW):
+    def __del__(self):  # its handle is none
+        pass
+
+
+def plan_of(library, workspace=16384):
+    plan = Plan.__new__(Plan)
+    plan._h, plan._L, plan._index, plan.device = ctypes.c_void_p(1), library, 0, torch.device("cuda", 0)
+    plan._bucket, plan._bucket_at, plan._workspace, plan._keep = None, None, workspace, []
+    return plan
+
+
+def control(monkeypatch):
+    """A Control whose memory is the host's."""
+    zeros = torch.zeros
+
+    class Memory:
+        def __init__(self, n):
+            self.t = zeros(n, dtype=torch.uint8)
+            self.is_cuda = True
+
+        def __getitem__(self, at):
+            m = Memory(0)
+            m.t = self.t[at]
+            return m
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+        def get_device(self):
+            return 0
+
+    monkeypatch.setattr(optim.torch, "zeros", lambda n, dtype, device: Memory(n))
+    c = optim.Control("cuda:0", lr=0.5, step=3)
+    monkeypatch.setattr(optim.torch, "zeros", zeros)
+    return c
+
+
+@pytest.mark.parametrize("stream", [None, 1234])
+def test_norm_takes_its_partial_sums_from_the_control(monkeypatch, stream):
+    """A call allocates nothing: memory from torch's allocator belongs to the current stream, and work
+    still queued there may use it while the call runs on another one.  The partial sums lie in the
+    Control, which is ordered between streams by its owner."""
+    ctrl, library = control(monkeypatch), Library()
+
+    def empty(*a, **k):
+        raise AssertionError("grad_norm_ allocates")
+
+    monkeypatch.setattr(optim.torch, "empty", empty)
+    monkeypatch.setattr(optim, "_current_stream", lambda index: 77)
+    plan = plan_of(library)
+    plan.grad_norm_(ctrl, max_norm=1.0, stream=stream)
+    (name, (_, bucket, scale, max_norm, at, ws, size, s)), = library.calls
+    assert (name, bucket, scale, max_norm, s) == ("hydra_adamw_grad_norm", None, 1.0, 1.0, stream or 77)
+    assert at == ctrl.ptr and ctrl.buffer.numel() == 64
+    memory = ctrl.buffer.untyped_storage()
+    assert size == 16384 and at + 64 <= ws and ws + size <= memory.data_ptr() + memory.nbytes() and ws % 8 == 0

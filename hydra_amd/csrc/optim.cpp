@@ -170,11 +170,9 @@ uint32_t head_of(const hydra_adamw_config_t& c, const hydra_adamw_tensor_t& t) {
   return (uint32_t)std::min<size_t>(best, t.n);
 }
 
-// Tiles of a tensor: at least one where there are elements.
-size_t tiles_of(size_t n, uint32_t head) {
-  if (n == 0) return 0;
-  return std::max<size_t>(1, (n - head + hydra::kOptTile - 1) / hydra::kOptTile);
-}
+// Tiles of a tensor, whatever its head: the norm's order of sums hangs on them, and on no address.  (The
+// step leaves the last one empty where the head takes its elements.)
+size_t tiles_of(size_t n) { return (n + hydra::kOptTile - 1) / hydra::kOptTile; }
 
 int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_tensor_t* tensors,
            size_t count, hydra_adamw** made) {
@@ -185,7 +183,7 @@ int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_ten
   size_t tiles = 0;
   for (size_t i = 0; i < count; i++) {
     if (int rc = check_tensor(i, *config, tensors[i], &written, &grads)) return rc;
-    tiles += tiles_of(tensors[i].n, head_of(*config, tensors[i]));
+    tiles += tiles_of(tensors[i].n);
   }
   if (tiles > kMaxTiles || count >= (size_t(1) << 31))
     return fail(HYDRA_ERR_INVALID, "too many elements for one plan: split it");
@@ -242,7 +240,7 @@ int create(int device, const hydra_adamw_config_t* config, const hydra_adamw_ten
     desc[i] = {static_cast<char*>(t.param), t.master, reinterpret_cast<uint64_t>(t.grad),
                static_cast<char*>(t.m), static_cast<char*>(t.v), t.m_scale, t.v_scale, t.n,
                t.lr_scale, t.weight_decay, tile, (uint32_t)i, head_of(*config, t), 0};
-    desc[i].tiles = (uint32_t)tiles_of(t.n, desc[i].head);
+    desc[i].tiles = (uint32_t)tiles_of(t.n);
     for (uint32_t k = 0; k < desc[i].tiles; k++) of_tile[tile++] = (uint32_t)i;
   }
   hipStream_t s = nullptr;

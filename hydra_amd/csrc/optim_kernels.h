@@ -16,9 +16,10 @@ constexpr uint32_t kMaxHead = 64;   // a head is one element per lane of one wav
 constexpr int kNormBlocks = 2048;   // workgroups (and partial sums) of the norm, at most
 
 // One tensor of a plan, in device memory.  `grad` counts from the bucket that a call gives (null:
-// an address).  Its tile k is number tile0 + k and holds the elements [head + k * kOptTile,
-// head + (k + 1) * kOptTile), the first one those before them too: `head` puts the vectors of as many
-// of its buffers as possible on their natural alignment, and their tiles on whole lines.
+// an address).  It has a tile for each kOptTile elements; tile k is number tile0 + k.  To the step it
+// holds the elements [head + k * kOptTile, head + (k + 1) * kOptTile), the first one those before them
+// too, the last one none at times: `head` puts the vectors of as many of its buffers as possible on
+// their natural alignment, and their tiles on whole lines.  To the norm: [k * kOptTile, (k + 1) * kOptTile).
 struct OptTensor {
   char* param;
   float* master;

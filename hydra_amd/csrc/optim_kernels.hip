@@ -251,7 +251,7 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
   Scalars k;
   if (!load_scalars(st, T, &k)) return;
   const uint64_t base = T.head + (uint64_t)(tile - T.tile0) * kOptTile;
-  const uint32_t left = (uint32_t)min(T.n - base, (uint64_t)kOptTile);
+  const uint32_t left = T.n > base ? (uint32_t)min(T.n - base, (uint64_t)kOptTile) : 0u;
   const gptr grad = global((const void*)(bucket + T.grad)) + base * sizeof(G);
   const gptr param = global(T.param) + base * sizeof(P), master = global(T.master) + base * 4;
   const gptr mm = global(T.m) + base * 4, vv = global(T.v) + base * 4;
@@ -513,8 +513,9 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
 
 // ---- the norm --------------------------------------------------------------------------------------
 // fp64 sums: no gradient's square overflows, and the sum is not finite exactly when some gradient
-// is not.  The order is the grid's, which the plan fixes: workgroup b sums a contiguous run of tiles,
-// and one workgroup adds the sums in a second launch (4.5 us, nearly all of it the launch; the
+// is not.  The order is that of the elements' numbers, whatever the addresses: a tensor's tiles count
+// from its first element, a tile's vectors go to the threads by their number, and workgroup b sums a
+// contiguous run of tiles, cut by the tensors' lengths alone.  One workgroup adds the sums in a second launch (4.5 us, nearly all of it the launch; the
 // workgroups counting their arrivals in the first one instead cost 9 us more for 1024 of them, 36
 // where the count also writes the caches back).  A small plan is one workgroup's, in one launch: that
 // takes 0.6 us for each tensor in turn and 0.05 for each tile (fp32; bf16 0.04), where two launches
@@ -567,13 +568,39 @@ __device__ __forceinline__ void add_squares(uint32_t w, double& sum) {
   }
 }
 
-// the thread's vector of `left` ones
-template <bool KEEP>
-__device__ __forceinline__ w4 vector_or_zero(gptr at, uint64_t left) {
-  w4 x = {0, 0, 0, 0};
-  if (threadIdx.x < left)
-    x = KEEP ? *(const GLOBAL w4*)(at + threadIdx.x * 16) : ldv<w4>(at, threadIdx.x * 16);
+// The thread's vector of `left` ones, at any alignment of its elements.  16-bit elements whose pairs
+// lie across memory's dwords (`odd`) are loaded by whole dwords from the second one on, and the first
+// one is the last half of the lane before (of its own load in a wave's first lane): 100 M bf16 elements
+// 37.4 us so, 44.4 by loads across the dwords, 36.3 at other offsets.
+struct Sixteen {
+  w4 d;
+  uint32_t first;
+};
+template <typename G, bool KEEP>
+__device__ __forceinline__ Sixteen load_sixteen(gptr at, uint64_t left, bool odd) {
+  Sixteen x{{0, 0, 0, 0}, 0};
+  if (threadIdx.x >= left) return x;
+  const uint32_t o = threadIdx.x * 16;
+  if (sizeof(G) == 4 || !odd) {
+    x.d = KEEP ? *(const GLOBAL w4*)(at + o) : ldv<w4>(at, o);
+    return x;
+  }
+  if (threadIdx.x + 1 < left) {
+    x.d = KEEP ? *(const GLOBAL w4*)(at + o + 2) : ldv<w4>(at, o + 2);
+  } else {  // nothing behind the last vector is read
+    for (int j = 0; j < 3; j++) x.d[j] = *(const GLOBAL uint32_t*)(at + o + 2 + 4 * j);
+    x.d[3] = *(const GLOBAL uint16_t*)(at + o + 14);
+  }
+  if ((threadIdx.x & 63) == 0) x.first = (uint32_t)*(const GLOBAL uint16_t*)(at + o) << 16;
   return x;
+}
+template <typename G>
+__device__ __forceinline__ w4 dwords_of(const Sixteen& x, bool odd) {
+  if (sizeof(G) == 4 || !odd) return x.d;
+  const uint32_t first =  // wave_shr:1
+      (uint32_t)__builtin_amdgcn_update_dpp((int)x.first, (int)x.d[3], 0x138, 0xf, 0xf, false);
+  return w4{__builtin_amdgcn_alignbit(x.d[0], first, 16), __builtin_amdgcn_alignbit(x.d[1], x.d[0], 16),
+            __builtin_amdgcn_alignbit(x.d[2], x.d[1], 16), __builtin_amdgcn_alignbit(x.d[3], x.d[2], 16)};
 }
 
 // 2048 workgroups, 32 waves per CU: 64 Mi fp32 42 us (6.4 TB/s), 397 bf16 tensors of 100 M elements
@@ -595,33 +622,30 @@ __global__ __launch_bounds__(BS) void k_norm(const OptTensor* tensors, const uin
   while (tile < last) {  // one tensor's share: [from, to)
     const OptTensor T = tensors[tile_tensor[tile]];
     const uint32_t first = tile - T.tile0, end = min(last - T.tile0, T.tiles);
-    const uint64_t from = first ? T.head + first * (uint64_t)kOptTile : 0;
-    const uint64_t to = min(T.head + end * (uint64_t)kOptTile, T.n);
-    const uint64_t addr = bucket + T.grad + from * sizeof(G), n = to - from;
-    // whole vectors from the first 16-byte boundary on; wave 0 takes what is before, wave 1 what is after
-    const uint32_t head = (uint32_t)min((uint64_t)((16 - (addr & 15)) & 15) / sizeof(G), n);
-    const uint64_t vecs = (n - head) / N;
-    const uint32_t tail = (uint32_t)(n - head - vecs * N);
-    const gptr ends = global((const void*)addr);
-    if (threadIdx.x < head) {
-      const double g = At<G>::load(ends, threadIdx.x);
-      sum = fma(g, g, sum);
-    } else if (threadIdx.x >= 64 && threadIdx.x - 64 < tail) {
-      const double g = At<G>::load(ends + (head + vecs * N) * sizeof(G), threadIdx.x - 64);
+    const uint64_t from = first * (uint64_t)kOptTile, n = min(end * (uint64_t)kOptTile, T.n) - from;
+    const uint64_t vecs = n / N;
+    const uint32_t tail = (uint32_t)(n - vecs * N);  // of the tensor's last tile
+    gptr at = global((const void*)(bucket + T.grad)) + from * sizeof(G);
+    if (threadIdx.x >= 64 && threadIdx.x - 64 < tail) {
+      const double g = At<G>::load(at + vecs * 16, threadIdx.x - 64);
       sum = fma(g, g, sum);
     }
-    gptr at = ends + head * sizeof(G);
     // one vector per thread and turn, the next one's load in flight while this one is summed
-    w4 x = vector_or_zero<KEEP>(at, vecs);
-    for (uint64_t left = vecs; left;) {
-      const uint64_t next = left > BS ? left - BS : 0;
-      at += BS * 16;
-      const w4 y = vector_or_zero<KEEP>(at, next);
+    auto add_all = [&](auto odd) {
+      Sixteen x = load_sixteen<G, KEEP>(at, vecs, odd);
+      for (uint64_t left = vecs; left;) {
+        const uint64_t next = left > BS ? left - BS : 0;
+        at += BS * 16;
+        const Sixteen y = load_sixteen<G, KEEP>(at, next, odd);
+        const w4 w = dwords_of<G>(x, odd);
 #pragma unroll
-      for (int j = 0; j < 4; j++) add_squares<G>(x[j], sum);
-      x = y;
-      left = next;
-    }
+        for (int j = 0; j < 4; j++) add_squares<G>(w[j], sum);
+        x = y;
+        left = next;
+      }
+    };
+    if (sizeof(G) == 2 && ((uint64_t)at & 2)) add_all(std::true_type{});
+    else add_all(std::false_type{});
     tile = T.tile0 + end;
   }
   sum = block_sum<BS>(sum, lds);

@@ -1,11 +1,12 @@
 """GPU tests of how a program calls the optimizer step: streams, captures, threads, alignments and
 sizes beyond one launch's or 32 bits (hydra_amd/optim.py); the operators' values are tested in
 test_gpu_optim.py."""
+import numpy as np
 import pytest
 
 import optim_ref as R
 from hydra_amd import optim
-from test_gpu_optim import Setup, f64
+from test_gpu_optim import Setup, dt, f64
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,91 @@ def test_capture_of_a_stream_that_is_not_current(gpu):
         torch.cuda.synchronize()
         assert torch.equal(a.p.buf, b.p.buf) and torch.equal(a.pm.buf, b.pm.buf) and torch.equal(ca.buffer, cb.buffer), k
         assert all((x == 255).all() for x in junk)
+
+
+def at_a_border(rng, n, kind):
+    """n gradients of type `kind` (in fp64) whose norm lies half way between two fp32 numbers to less than
+    a step of fp64: sums of their squares in different orders round to different norms."""
+    import torch
+
+    def toward_zero(x):
+        y = torch.tensor(x, dtype=torch.float64).to(dt(kind)).double().item()
+        if y <= x:
+            return y
+        return torch.nextafter(torch.tensor(y).to(dt(kind)), torch.zeros((), dtype=dt(kind))).double().item()
+
+    ends = 6 if kind == "f32" else 16  # each leaves at most 2^-9 of the rest
+    g = torch.from_numpy(rng.normal(0, 1, n)).to(dt(kind)).double().numpy()
+    g[-ends:] = 0.0
+    total = (g.astype(np.longdouble) ** 2).sum()
+    step = float(np.spacing(np.float32(np.sqrt(float(total)))))
+    border = np.longdouble(float(np.float32(np.sqrt(float(total)))) + 2.5 * step)
+    rest = border * border - total
+    for i in range(ends):
+        g[n - ends + i] = toward_zero(float(np.sqrt(rest)))
+        rest -= np.longdouble(g[n - ends + i]) ** 2
+        assert rest >= 0
+    assert rest < border * border * 2.0 ** -54
+    return g
+
+
+@pytest.mark.parametrize("grad", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("sizes", [[5000], [200_003], [20_001, 70, 0, 1025, 66_000], [1, 1087, 3, 2049]])
+def test_norm_bits_at_any_address(gpu, sizes, grad):
+    """The same gradients at other addresses, in plans whose weights and moments lie elsewhere, in other
+    buckets, and in a plan of gradients alone: the same bits."""
+    import torch
+
+    total, gaps = sum(sizes), (0, 1, 2, 3, 5, 8, 31)
+
+    def views(at, gap, dtype):
+        out, buf = [], torch.zeros(total + 64 + gap * len(sizes), dtype=dtype, device=gpu)
+        for n in sizes:
+            out.append(buf[at:at + n])
+            at += n + gap
+        return out
+
+    layouts = []
+    for gap in gaps:
+        grads = views(gap, gap, dt(grad))
+        layouts.append((optim.AdamW(None, grads), grads, None))
+        p, m, v = (views(gap + i * 7, (gap + i) % 5, torch.float32) for i in range(3))
+        grads = views(31 - gap, gap, dt(grad))
+        layouts.append((optim.AdamW(p, grads, m, v), grads, None))
+    bucket = torch.zeros(total, dtype=dt(grad), device=gpu)
+    grads, at = [], 0
+    for n in sizes:
+        grads.append(bucket[at:at + n])
+        at += n
+    in_bucket = optim.AdamW(None, grads, bucket=bucket)
+    for gap in gaps:
+        layouts.append((in_bucket, None, torch.zeros(total + 64, dtype=dt(grad), device=gpu)[gap:gap + total]))
+    rng = np.random.default_rng(7)
+    ctrl = optim.Control(gpu)
+    for draw in range(24):
+        g = at_a_border(rng, total, grad)
+        values = torch.from_numpy(g).to(dt(grad)).to(gpu)
+        got = set()
+        for plan, grads, other in layouts:
+            if other is not None:
+                other.copy_(values)
+            else:
+                for x, y in zip(grads, values.split(sizes)):
+                    x.copy_(y)
+            plan.grad_norm_(ctrl, bucket=other)
+            got.add(ctrl.norm.item())
+        norm, _ = R.norm64([g], 1.0, 0.0)
+        assert abs(got.pop() - norm) <= (R.U32 + 2.0 ** -28) * norm and not got, (draw, got)
+
+
+@pytest.mark.parametrize("gap", [0, 1, 2, 3, 5, 8, 16, 31])
+def test_step_of_heads_and_last_tiles(gpu, gap):
+    """Lengths a little above whole tiles, at offsets whose heads leave the last tile without elements."""
+    sizes = [1025, 1026, 2049, 1024 + 31, 1024 + 32, 1024 + 63, 4096 + 64, 1024, 2048, 31, 63, 64]
+    s = Setup(gpu, sizes, "bf16", True, "bf16", seed=gap, pad=gap)
+    t = Setup(gpu, sizes, seed=gap, pad=gap)
+    for x in (s, t):
+        before = x.state()
+        x.plan.step_(lr=1e-3, step=3)
+        x.compare(before, x.state(), lr=1e-3, t=3)
+        x.guards()

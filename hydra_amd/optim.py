@@ -19,8 +19,8 @@ zeroed to start with, and a seed that stays the same for the whole training:
 """
 from __future__ import annotations
 
+import collections
 import ctypes
-import sys
 
 import numpy as np
 import torch
@@ -28,15 +28,13 @@ import torch
 from . import _lib
 from ._lib import HydraError, check
 
-_is_finalizing = sys.is_finalizing
-
 MOMENT_BLOCK = 256  # elements that share one scale of an 8-bit moment
 _WORKSPACE = 16384  # HYDRA_ADAMW_WORKSPACE_MAX (include/hydra_optim.h)
 _CODES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
 # the current stream's handle by device index (torch.cuda.current_stream builds a Stream object
 # around it: 2 us, as long as a small step's kernel runs)
 _current_stream = torch._C._cuda_getCurrentRawStream
-_left = []  # handles of plans dropped during a capture: released when the next plan is made
+_left = collections.deque()  # handles of dropped plans: released when the next plan is made or closed
 
 
 def moment_scales(n: int) -> int:
@@ -57,6 +55,15 @@ def _list(x) -> list:
 
 def _refuse(msg: str):
     raise HydraError(_lib.ERR_INVALID, msg)
+
+
+def _release_left() -> None:
+    while True:
+        try:
+            h = _left.popleft()  # (another thread may have taken the last one)
+        except IndexError:
+            return
+        _lib.lib().hydra_adamw_destroy(h)
 
 
 class Control:
@@ -91,14 +98,18 @@ class AdamW:
     grad_norm_ alone.  bucket: a 1-d tensor whose views the grads are; each call may then name
     another bucket of that layout (two buckets in turn, one being reduced while the other is
     stepped).  The plan keeps the tensors alive; a graph that holds its calls does not.  Calls write
-    the tensors past autograd: nothing that a backward pass still needs may be among them."""
+    the tensors past autograd: nothing that a backward pass still needs may be among them.
+
+    Plans are made and closed while no thread captures a stream.  One that is dropped without close()
+    waits with its device tables (88 bytes a tensor and 4 for 1024 elements) until the next one is made or
+    closed, so plans may be dropped at any time."""
 
     def __init__(self, params, grads, m=None, v=None, *, master=None, m_scale=None, v_scale=None,
                  betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0,
                  bucket=None):
         self._h = ctypes.c_void_p()
-        while _left and not torch.cuda.is_current_stream_capturing():
-            _lib.lib().hydra_adamw_destroy(_left.pop())
+        if _left and not torch.cuda.is_current_stream_capturing():
+            _release_left()
         grads = _list(grads)
         if not grads:
             _refuse("AdamW: no tensors")
@@ -233,23 +244,18 @@ class AdamW:
             check(rc)
 
     def close(self) -> None:
-        """Waits for the device's work, then releases the plan (not while a stream is captured)."""
+        """Waits for the device's work, then releases the plan."""
         if self._h:
-            _lib.lib().hydra_adamw_destroy(self._h)
+            _left.append(self._h)
             self._h = ctypes.c_void_p()
             self._keep = []
+        _release_left()
 
     def __del__(self):
-        # no HIP calls while the interpreter is finalizing (this module's names may be gone by then)
-        if _is_finalizing is None or _is_finalizing():
-            return
-        try:
-            if self._h and torch.cuda.is_current_stream_capturing():
-                _left.append(self._h)  # waiting for the device would end the capture
-                return
-            self.close()
-        except Exception:
-            pass
+        # releasing waits for the device, which would end a capture of any thread's: that is left to
+        # the next plan made or closed (while the interpreter is finalizing, the deque may be gone)
+        if _left is not None and self._h:
+            _left.append(self._h)
 
 
 def _moments(m, v, m8, m_scale, v8, v_scale):

@@ -1,6 +1,5 @@
 """How hydra_amd.optim makes its calls, without a GPU: plans whose library is a stand-in."""
 import ctypes
-import types
 
 import pytest
 
@@ -80,3 +79,60 @@ def test_norm_takes_its_partial_sums_from_the_control(monkeypatch, stream):
     assert at == ctrl.ptr and ctrl.buffer.numel() == 64
     memory = ctrl.buffer.untyped_storage()
     assert size == 16384 and at + 64 <= ws and ws + size <= memory.data_ptr() + memory.nbytes() and ws % 8 == 0
+
+
+def left():
+    return [h.value for h in optim._left]
+
+
+def test_a_dropped_plan_waits(monkeypatch):
+    """Dropping a plan calls nothing: releasing it waits for the device, which would end a capture that
+    any thread makes.  The next plan that is made or closed releases it, once."""
+    library = Library()
+    monkeypatch.setattr(optim._lib, "lib", lambda: library)
+    monkeypatch.setattr(optim.torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert left() == []
+    plan = optim.AdamW.__new__(optim.AdamW)
+    plan._h, plan._keep = ctypes.c_void_p(11), []
+    del plan
+    assert library.calls == [] and left() == [11]
+    with pytest.raises(optim.HydraError, match="no tensors"):
+        optim.AdamW([], [], [], [])
+    assert [(name, h.value) for name, (h,) in library.calls] == [("hydra_adamw_destroy", 11)] and left() == []
+    plans = [optim.AdamW.__new__(optim.AdamW) for _ in range(2)]
+    for i, plan in enumerate(plans):
+        plan._h, plan._keep = ctypes.c_void_p(20 + i), []
+    del library.calls[:], plan
+    last = plans.pop()
+    del plans[0]
+    last.close()
+    last.close()
+    del last
+    assert sorted(h.value for _, (h,) in library.calls) == [20, 21] and left() == []
+
+
+def test_plans_left_during_a_capture_stay(monkeypatch):
+    library = Library()
+    monkeypatch.setattr(optim._lib, "lib", lambda: library)
+    monkeypatch.setattr(optim.torch.cuda, "is_current_stream_capturing", lambda: True)
+    optim._left.append(ctypes.c_void_p(5))
+    with pytest.raises(optim.HydraError, match="no tensors"):
+        optim.AdamW([], [], [], [])
+    assert library.calls == [] and left() == [5]
+    optim._left.clear()
+
+
+def test_two_threads_release_at_once(monkeypatch):
+    """The other thread takes the last one between the look and the taking."""
+    library = Library()
+    monkeypatch.setattr(optim._lib, "lib", lambda: library)
+
+    def capturing():
+        optim._left.clear()
+        return False
+
+    monkeypatch.setattr(optim.torch.cuda, "is_current_stream_capturing", capturing)
+    optim._left.append(ctypes.c_void_p(5))
+    with pytest.raises(optim.HydraError, match="no tensors"):
+        optim.AdamW([], [], [], [])
+    assert library.calls == []

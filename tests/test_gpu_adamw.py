@@ -158,3 +158,43 @@ def test_step_of_heads_and_last_tiles(gpu, gap):
         x.plan.step_(lr=1e-3, step=3)
         x.compare(before, x.state(), lr=1e-3, t=3)
         x.guards()
+
+
+def test_a_plan_dropped_while_another_thread_captures(gpu):
+    """The capture lives on, and the graph does what eager calls do."""
+    import threading
+
+    import torch
+
+    a, b = (Setup(gpu, [70_000, 3], seed=41) for _ in range(2))
+    ca, cb = (optim.Control(gpu, lr=1e-3) for _ in range(2))
+    dropped, graph, side = [Setup(gpu, [10], seed=1)], torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    begun, gone, errors = threading.Event(), threading.Event(), []
+
+    def capture():
+        try:
+            with torch.cuda.graph(graph, stream=side):
+                a.plan.grad_norm_(ca, max_norm=0.1)
+                begun.set()
+                gone.wait(30)
+                a.plan.step_(ctrl=ca)
+        except Exception as e:
+            errors.append(e)
+            begun.set()
+
+    t = threading.Thread(target=capture)
+    t.start()
+    begun.wait(30)
+    dropped.clear()
+    gone.set()
+    t.join()
+    assert not errors, errors
+    for k in range(3):
+        graph.replay()
+        b.plan.grad_norm_(cb, max_norm=0.1)
+        b.plan.step_(ctrl=cb)
+        torch.cuda.synchronize()
+        assert torch.equal(a.p.buf, b.p.buf) and torch.equal(ca.buffer, cb.buffer), k
+    assert len(optim._left) > 0
+    optim.AdamW(None, [b.g.views[0]]).close()
+    assert len(optim._left) == 0

@@ -330,18 +330,19 @@ __device__ __forceinline__ uint32_t add_high16(uint32_t c, uint32_t r) {
   asm("v_mad_u32_u16 %0, %1, 8, %2 op_sel:[1,0,0,0]" : "=v"(d) : "v"(r), "v"(c));
   return d;
 }
-// The square root of v >= 0, not denormal, rounded as sqrtf rounds it, in 8 issue slots instead of 17:
-// the reciprocal root's estimate s, then s + (v - s^2) / (2 s) (all 2^24 values of [1, 4) checked
-// against sqrtf; below 2^-98 the rest v - s^2 itself is rounded, and 1 ulp may be off).  A denormal
-// becomes something above 0 and below 2^-62; what is not finite, something not finite.
+// The square root of v in [0, 2^28], rounded as sqrtf rounds it (all of them checked against it), in 10
+// issue slots instead of 17: of w = v * 2^96, which is normal and whose w - s^2 is exact, the reciprocal
+// root's estimate s, then s + (w - s^2) / (2 s).  What lies above or is not finite becomes something not
+// below 2^14, or a NaN.
 __device__ __forceinline__ float plain_sqrt(float v) {
-  const float r = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f));
-  const float s = v * r;
-  return fmaf(fmaf(-s, s, v), 0.5f * r, s);
+  const float w = v * 0x1p96f;
+  const float r = __builtin_amdgcn_rsqf(fmaxf(w, 0x1p-126f));
+  const float s = w * r;
+  return fmaf(fmaf(-s, s, w), 0.5f * r, s) * 0x1p-48f;
 }
 // What a block's largest magnitude (its bits) has to be for the encoders below: 2^-112 / scale is
-// normal, and every value is finite.  sqrt v also 0, or not below 2^-43: what plain_sqrt makes of
-// denormals lies under the smallest byte then.
+// normal, and every value is finite.  sqrt v also 0, or not below 2^-43: under such a one a v of fewer
+// than 256 of fp32's smallest steps has the byte 1, and a minimum with its bits leaves every byte.
 __device__ __forceinline__ bool plain_m(uint32_t top) { return top < fbits(0x1p14f); }
 __device__ __forceinline__ bool plain_root(uint32_t top) {
   return top == 0 || top - fbits(0x1p-43f) < fbits(0x1p14f) - fbits(0x1p-43f);
@@ -380,8 +381,8 @@ __device__ __forceinline__ float uniform(float x, int lane) {
 // quotient in p's update the kernel took 170 us instead of 164).  The bytes are those of the documented
 // operations, each rounded to fp32.  Decoding is short where no byte stands for something not finite
 // and both old scales are below 2^15 (2^112 * scale is finite: one product per value).  The rest is
-// short where the block is plain (above) and eps lies in [2^-40, 2^60]: eps hides what plain_sqrt
-// does not see, and the quotient is a product with the hardware's reciprocal (2 ulp).
+// short where the block is plain (above) and eps lies in [2^-40, 2^60]: the quotient is then a product
+// with the hardware's reciprocal (2 ulp), both of them normal.
 template <typename P, typename G, bool MASTER>
 __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr m8, gptr v8,
                                        gptr ms, gptr vs, uint32_t left, uint32_t lane,

@@ -449,7 +449,7 @@ __device__ __forceinline__ void block8(gptr master, gptr param, gptr grad, gptr 
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const float denom = fmaf(root[j], k.isb2, k.eps);
-      p[j] = fmaf(m[j] * -k.size, __builtin_amdgcn_rcpf(denom), p[j] * k.decay);
+      p[j] = fmaf(m[j] * __builtin_amdgcn_rcpf(denom), -k.size, p[j] * k.decay);
     }
     scale = moment_scale(bitsf(top));
     const float inv = plain_inv(scale);

@@ -52,3 +52,13 @@ def test_weights_of_small_squares(gpu, low, high, eps, b2):
     g = squares(np.random.default_rng(3), 64, b2, low, high)
     (p, *_), m, v = step(gpu, g, eps=eps, b2=b2)
     weights(p, m, v, lr=1e-3, t=1, eps=eps, b2=b2, roundings=6)
+
+
+@pytest.mark.parametrize("lr", [1e-12, 1e-3, 1e3])
+@pytest.mark.parametrize("size", [2.0 ** -97, 2.0 ** -60, 1.0])
+def test_weights_of_small_updates(gpu, size, lr):
+    """The quotient comes before its product with the rate, as documented: m times a small rate alone
+    would be denormal."""
+    g = (np.random.default_rng(5).normal(0, 1, 4096) * size).astype(F)
+    (p, *_), m, v = step(gpu, g, lr=lr)
+    weights(p, m, v, lr=lr, t=1, eps=1e-8, b2=0.999, roundings=6)

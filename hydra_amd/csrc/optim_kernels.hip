@@ -26,7 +26,8 @@ namespace {
 // ---- 8-bit moments -------------------------------------------------------------------------------
 // The code of t in [0, 1.875] is the top of its fp32 bits once the exponent is rebased to a 4-bit
 // one: t * 2^-112 has exponent field 15 for t in [1, 2), and below 2^-14 it is an fp32 subnormal,
-// so the gradual underflow costs nothing.  Adding r below the cut before shifting rounds: 16
+// so the gradual underflow costs nothing: x / s is then a multiple of 2^-37, rounded once from the
+// product with fp32's 1 / s.  Adding r below the cut before shifting rounds: 16
 // random bits stochastically (the neglected rest of the dropped bits shifts the probability by at
 // most 2^-16), 0x8000 to nearest.  Largest code: 127 (m) and 254 (sqrt v), both 1.875.
 constexpr float kTop = 1.0f / 1.875f;
@@ -40,14 +41,19 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < INFINITY ? a : 0.0f;
 }
 
+// a * inv * 2^-112 rounded once, whatever inv is (in fp64 the products are exact)
+__device__ __forceinline__ uint32_t rebased(float a, float inv) {
+  return fbits((float)((double)a * inv * 0x1p-112));
+}
+
 __device__ __forceinline__ uint32_t encode_m(float m, float inv, uint32_t r16) {
   const float a = fabsf(m);
-  const uint32_t c = min((fbits(a * inv * 0x1p-112f) + (r16 << 4)) >> 20, 127u);
+  const uint32_t c = min((rebased(a, inv) + (r16 << 4)) >> 20, 127u);
   if (!(a < INFINITY)) return 0x80u;
   return c ? c | (m < 0.0f ? 0x80u : 0u) : 0u;
 }
 __device__ __forceinline__ uint32_t encode_root(float root, float inv, uint32_t r16) {
-  const uint32_t c = min((fbits(root * inv * 0x1p-112f) + (r16 << 3)) >> 19, 254u);
+  const uint32_t c = min((rebased(root, inv) + (r16 << 3)) >> 19, 254u);
   if (!(root < INFINITY)) return 255u;
   return root > 0.0f ? max(c, 1u) : 0u;
 }
@@ -347,7 +353,7 @@ __device__ __forceinline__ bool plain_m(uint32_t top) { return top < fbits(0x1p1
 __device__ __forceinline__ bool plain_root(uint32_t top) {
   return top == 0 || top - fbits(0x1p-43f) < fbits(0x1p14f) - fbits(0x1p-43f);
 }
-// 2^-112 / scale (0 for an empty block)
+// 2^-112 / scale (0 for an empty block): exact, so a product with it is rounded as in `rebased`
 __device__ __forceinline__ float plain_inv(float scale) { return moment_inv(scale) * 0x1p-112f; }
 // The bytes of four values of plain blocks; add(c, j) rounds c by the random bits of element j.
 template <typename F>

@@ -37,9 +37,10 @@ extern "C" {
  * with Fk the float of 4 exponent bits and k mantissa bits whose largest power of two is 1:
  * Fk(c) = c * 2^-(14 + k) for c < 2^k, else 2^((c >> k) - 15) * (1 + (c mod 2^k) / 2^k).  The byte
  * of a v above zero is at least 1, so no step divides by eps alone where fp32 holds v at all.  m, v
- * and the bytes come from the operations above, each rounded to fp32 (x = |value| * (1 / s)); the
- * quotient in p's update is within 2 units in the last place, and its product with lr' * c1 may not be
- * rounded before the difference.
+ * and the bytes come from the operations above, each rounded to fp32; the magnitude over s is the
+ * product with fp32's 1 / s, rounded to fp32 or, below 2^-14, to a multiple of 2^-37.  The quotient in
+ * p's update is within 2 units in the last place, and its product with lr' * c1 may not be rounded
+ * before the difference.
  * A step rounds its new moments stochastically: with x the magnitude over s, the two bytes around
  * x are taken with probabilities that make the mean x, by 16 random bits for each moment from a
  * 32-bit hash of (seed, t, the tensor's place in the plan, i) -- the same bits on every run and

@@ -522,13 +522,14 @@ __global__ __launch_bounds__(kOptBlock) void k_adamw8(const OptTensor* tensors,
 // fp64 sums: no gradient's square overflows, and the sum is not finite exactly when some gradient
 // is not.  The order is that of the elements' numbers, whatever the addresses: a tensor's tiles count
 // from its first element, a tile's vectors go to the threads by their number, and workgroup b sums a
-// contiguous run of tiles, cut by the tensors' lengths alone.  One workgroup adds the sums in a second launch (4.5 us, nearly all of it the launch; the
-// workgroups counting their arrivals in the first one instead cost 9 us more for 1024 of them, 36
-// where the count also writes the caches back).  A small plan is one workgroup's, in one launch: that
-// takes 0.6 us for each tensor in turn and 0.05 for each tile (fp32; bf16 0.04), where two launches
-// take 6.9 (1 tensor of 4 tiles 3.8 us, of 64 5.9, of 96 7.4; 6 tensors of 4 tiles 6.1, 8 7.4).
+// contiguous run of tiles, cut by the tensors' lengths alone.  One workgroup adds the sums in a second
+// launch (4.5 us, nearly all of it the launch; the workgroups counting their arrivals in the first one
+// instead cost 9 us more for 1024 of them, 36 where the count also writes the caches back).  A small plan
+// is one workgroup's, in one launch.  That takes, beside 6.5 to 6.7 us for two launches at every one of
+// these sizes: one fp32 tensor of 16 tiles 3.8, 48 5.1, 64 5.9, 80 6.7, 96 7.5 (bf16: 80 5.6, 112 6.7);
+// 4 tensors of a tile 4.1, 8 5.8, 9 6.2, 10 6.7, 12 7.5; 7 of 4 tiles 5.4.
 constexpr int kNormAloneBlock = 1024;
-bool norm_alone(const OptTable& t) { return t.tiles + 12 * (uint64_t)t.filled <= 96; }
+bool norm_alone(const OptTable& t) { return t.tiles + 8 * (uint64_t)t.filled <= 88; }
 
 template <int BS>
 __device__ __forceinline__ double block_sum(double x, double* lds) {

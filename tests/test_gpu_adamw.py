@@ -147,6 +147,26 @@ def test_norm_bits_at_any_address(gpu, sizes, grad):
         assert abs(got.pop() - norm) <= (R.U32 + 2.0 ** -28) * norm and not got, (draw, got)
 
 
+@pytest.mark.parametrize("sizes,launches", [([80 * 1024], 1), ([80 * 1024 + 1], 2), ([9] * 9 + [0], 1), ([9] * 10, 2),
+                                            ([4096] * 7, 1), ([4096] * 8, 2), ([], 1)])
+def test_norm_in_one_launch_or_two(gpu, sizes, launches):
+    """Both sides of the border: the same definition."""
+    import torch
+
+    sizes = sizes or [0]
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(9)
+    grads = [torch.randn(n, generator=gen, device=gpu) for n in sizes]
+    plan, ctrl = optim.AdamW(None, grads), optim.Control(gpu, step=5)
+    assert (plan._workspace == 0) == (launches == 1)
+    for k in range(3):
+        plan.grad_norm_(ctrl, max_norm=0.5, grad_scale=0.25)
+        norm, mult = R.norm64([f64(x) for x in grads], 0.25, 0.5)
+        assert abs(ctrl.norm.item() - norm) <= (R.U32 + 2.0 ** -28) * norm
+        assert abs(ctrl.mult.item() - mult) <= (R.U32 + 2.0 ** -28) * mult
+        assert (ctrl.step.item(), ctrl.skip.item()) == (6 + k, 0)
+
+
 @pytest.mark.parametrize("gap", [0, 1, 2, 3, 5, 8, 16, 31])
 def test_step_of_heads_and_last_tiles(gpu, gap):
     """Lengths a little above whole tiles, at offsets whose heads leave the last tile without elements."""

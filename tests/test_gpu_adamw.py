@@ -218,3 +218,73 @@ def test_a_plan_dropped_while_another_thread_captures(gpu):
     assert len(optim._left) > 0
     optim.AdamW(None, [b.g.views[0]]).close()
     assert len(optim._left) == 0
+
+
+def repeated(x, n):
+    """n elements that repeat x."""
+    import torch
+
+    out = torch.empty(n, dtype=x.dtype, device=x.device)
+    for at in range(0, n, 1 << 28):
+        part = out[at:at + (1 << 28)]
+        part.copy_(x.repeat(-(-part.numel() // x.numel()))[: part.numel()])
+    return out
+
+
+def test_conversions_beyond_one_launch(gpu):
+    """More elements than one launch takes (2^30): a stretch's bytes and values are those of the stretch
+    alone, on both sides of the border and at the ragged end."""
+    import torch
+
+    n = (1 << 30) + 256 * 5 + 77
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(3)
+    level = torch.exp2(torch.randint(-20, 4, (1 << 20,), generator=gen, device=gpu).float())
+    m = repeated(torch.randn(1 << 20, generator=gen, device=gpu) * level, n)
+    v = repeated((torch.randn(1 << 20, generator=gen, device=gpu) * level) ** 2, n)
+    m[1 << 30] = 1e3  # the second launch's first block and the last one are like no other
+    v[-1] = 1e6
+    rows = optim.moment_scales(n)
+    m8, v8 = (torch.full((n + 1,), 77, dtype=torch.uint8, device=gpu) for _ in "mv")
+    ms, vs = (torch.full((rows + 1,), 7.0, device=gpu) for _ in "mv")
+    optim.moments8_encode_(m8[:n], ms[:rows], v8[:n], vs[:rows], m, v)
+    mo, vo = (torch.full((n + 1,), 7.0, dtype=torch.bfloat16, device=gpu) for _ in "mv")
+    optim.moments8_decode_(mo[:n], vo[:n], m8[:n], ms[:rows], v8[:n], vs[:rows])
+    for x in (m8, v8, ms, vs, mo, vo):
+        assert x[-1].item() in (77, 7.0)
+    for at, end in ((0, 4096), ((1 << 30) - 2048, (1 << 30) + 1024), ((1 << 30) - 256, 1 << 30), (1 << 30, n), (n // 256 * 256, n)):
+        k, first, last = end - at, at // 256, -(-end // 256)
+        a8, b8 = (torch.zeros(k, dtype=torch.uint8, device=gpu) for _ in "mv")
+        sa, sb = (torch.zeros(last - first, device=gpu) for _ in "mv")
+        optim.moments8_encode_(a8, sa, b8, sb, m[at:end], v[at:end])
+        ao, bo = (torch.zeros(k, dtype=torch.bfloat16, device=gpu) for _ in "mv")
+        optim.moments8_decode_(ao, bo, a8, sa, b8, sb)
+        for got, want in ((m8[at:end], a8), (v8[at:end], b8), (ms[first:last], sa), (vs[first:last], sb), (mo[at:end], ao), (vo[at:end], bo)):
+            assert torch.equal(got, want), (at, end)
+    assert ms[1 << 22].item() > 500 and vs[rows - 1].item() > 500
+
+
+def test_step_beyond_32_bits(gpu):
+    """fp32 moments of more than 2^32 elements, at an odd offset."""
+    import torch
+
+    n = (1 << 32) + 4096 * 3 + 77
+    bf = torch.bfloat16
+    pattern = (torch.randn(1 << 20, device=gpu) * 0.01).to(bf)
+    g = repeated(pattern, n + 3)[3:]
+    p = torch.zeros(n + 4, dtype=bf, device=gpu)
+    m, v = (torch.zeros(n + 2, device=gpu) for _ in "mv")
+    plan = optim.AdamW([p[3:n + 3]], [g], [m[1:n + 1]], [v[1:n + 1]], weight_decay=0.0)
+    ctrl = optim.Control(gpu, lr=0.5)
+    plan.grad_norm_(ctrl)
+    total = float((f64(pattern) ** 2).sum()) * 4096 + float((f64(g[(1 << 32) - 3:]) ** 2).sum())
+    assert abs(ctrl.norm.item() - np.sqrt(total)) <= np.sqrt(total) * (R.U32 + 2.0 ** -30)
+    plan.step_(ctrl=ctrl)
+    for at in (0, (1 << 30) - 100, (1 << 31) - 512, (1 << 32) - 512, n - 3000):
+        end = min(n, at + 5120)
+        x = f64(g[at:end])
+        zero = np.zeros(x.size)
+        (want, wm, wv), (ep, em, ev) = R.step64(zero, x, zero, zero, lr=0.5, t=1)
+        assert (np.abs(f64(m[at + 1:end + 1]) - wm) <= em).all() and (np.abs(f64(v[at + 1:end + 1]) - wv) <= ev).all(), at
+        assert (np.abs(f64(p[at + 3:end + 3]) - want) <= ep + 2.0 ** -8 * (np.abs(want) + ep)).all(), at
+    assert (p[:3] == 0).all() and p[n + 3] == 0 and all(x[0] == 0 and x[n + 1] == 0 for x in (m, v))

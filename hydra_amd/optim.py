@@ -29,6 +29,7 @@ from . import _lib
 from ._lib import HydraError, check
 
 MOMENT_BLOCK = 256  # elements that share one scale of an 8-bit moment
+_SEEDS = (1 << 64) - 1
 _WORKSPACE = 16384  # HYDRA_ADAMW_WORKSPACE_MAX (include/hydra_optim.h)
 _CODES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
 # the current stream's handle by device index (torch.cuda.current_stream builds a Stream object
@@ -242,6 +243,8 @@ class AdamW:
             rc = self._L.hydra_adamw_step(h, b, lr, step, grad_scale, seed, s)
         if rc:
             check(rc)
+        if not 0 <= seed <= _SEEDS:
+            _refuse("step_: a seed has 64 bits")
 
     def close(self) -> None:
         """Waits for the device's work, then releases the plan."""

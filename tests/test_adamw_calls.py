@@ -136,3 +136,18 @@ def test_two_threads_release_at_once(monkeypatch):
     with pytest.raises(optim.HydraError, match="no tensors"):
         optim.AdamW([], [], [], [])
     assert library.calls == []
+
+
+@pytest.mark.parametrize("seed", [-1, 1 << 64, (1 << 64) + 5])
+def test_seeds_beyond_64_bits_are_refused(monkeypatch, seed):
+    """2^64 would wrap to 0, which rounds to nearest."""
+    library, ctrl = Library(), control(monkeypatch)
+    monkeypatch.setattr(optim, "_current_stream", lambda index: 77)
+    plan = plan_of(library)
+    for kw in (dict(lr=1e-3, step=1), dict(ctrl=ctrl)):
+        with pytest.raises(optim.HydraError, match="seed"):
+            plan.step_(seed=seed, **kw)
+    assert library.calls == []
+    plan.step_(lr=1e-3, step=1, seed=(1 << 64) - 1)
+    plan.step_(ctrl=ctrl, seed=0)
+    assert [name for name, _ in library.calls] == ["hydra_adamw_step", "hydra_adamw_step_ctrl"]

@@ -88,6 +88,15 @@ class Control:
         self.lr.fill_(lr)
         self.step.fill_(step)
 
+    def __reduce__(self):  # a copy, also by way of a file, has memory of its own
+        return _control_of, (self.buffer,)
+
+
+def _control_of(buffer) -> Control:
+    c = Control(buffer.device)
+    c.buffer.copy_(buffer)
+    return c
+
 
 class AdamW:
     """A plan (hydra_adamw_t): the tensors that are stepped together, laid out once.
@@ -206,6 +215,9 @@ class AdamW:
             _refuse("AdamW: the bucket is shorter than the plan's")
         return bucket.data_ptr()
 
+    def __reduce__(self):
+        _refuse("AdamW: a plan cannot be copied: make another over the tensors of the copy")
+
     def _closed(self):
         _refuse("AdamW: the plan is closed")
 
@@ -231,6 +243,8 @@ class AdamW:
         h = self._h or self._closed()
         b = self._bucket_ptr(bucket) if self._bucket is not bucket else self._bucket_at
         s = _current_stream(self._index) if stream is None else stream
+        if not 0 <= seed <= _SEEDS:
+            _refuse("step_: a seed has 64 bits")
         if ctrl is not None:
             if lr is not None or step is not None or grad_scale != 1.0:
                 _refuse("step_: lr, step and grad_scale come from ctrl")
@@ -243,8 +257,6 @@ class AdamW:
             rc = self._L.hydra_adamw_step(h, b, lr, step, grad_scale, seed, s)
         if rc:
             check(rc)
-        if not 0 <= seed <= _SEEDS:
-            _refuse("step_: a seed has 64 bits")
 
     def close(self) -> None:
         """Waits for the device's work, then releases the plan."""

@@ -151,3 +151,13 @@ def test_seeds_beyond_64_bits_are_refused(monkeypatch, seed):
     plan.step_(lr=1e-3, step=1, seed=(1 << 64) - 1)
     plan.step_(ctrl=ctrl, seed=0)
     assert [name for name, _ in library.calls] == ["hydra_adamw_step", "hydra_adamw_step_ctrl"]
+
+
+def test_plans_are_not_copied():
+    """A copy would hold the first one's handle, and release it again."""
+    import copy
+    import pickle
+
+    for make in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(optim.HydraError, match="copied"):
+            make(plan_of(Library()))

@@ -288,3 +288,22 @@ def test_step_beyond_32_bits(gpu):
         assert (np.abs(f64(m[at + 1:end + 1]) - wm) <= em).all() and (np.abs(f64(v[at + 1:end + 1]) - wv) <= ev).all(), at
         assert (np.abs(f64(p[at + 3:end + 3]) - want) <= ep + 2.0 ** -8 * (np.abs(want) + ep)).all(), at
     assert (p[:3] == 0).all() and p[n + 3] == 0 and all(x[0] == 0 and x[n + 1] == 0 for x in (m, v))
+
+
+def test_a_copied_control_has_its_own_memory(gpu):
+    """The calls go to the copy's addresses, not to the first one's."""
+    import copy
+    import pickle
+
+    import torch
+
+    grads = [torch.randn(n, device=gpu) for n in (200_000, 5)]
+    plan, first = optim.AdamW(None, grads), optim.Control(gpu, lr=0.25, step=7)
+    plan.grad_norm_(first)
+    before = first.buffer.clone()
+    for make in (copy.copy, copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))):
+        c = make(first)
+        assert torch.equal(c.buffer, before) and c.ptr == c.buffer.data_ptr() != first.ptr
+        plan.grad_norm_(c)
+        assert (c.step.item(), c.lr.item(), c.norm.item()) == (9, 0.25, first.norm.item())
+        assert torch.equal(first.buffer, before)

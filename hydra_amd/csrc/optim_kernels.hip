@@ -4,8 +4,8 @@
 // Every kernel here is a stream over HBM: AdamW moves 28 B per element with fp32 moments and 16
 // with 8-bit ones, the norm 4 or 2, the conversions of both moments 10 (from fp32) and 6 (to bf16).
 // No reuse, no MFMA; what bounds them is the rate at which HBM takes mixed reads and writes (a copy
-// 6.3 TB/s, reads alone 6.8), and for 8-bit moments nearly the vector units too (60 issue slots per
-// element, 103 us for 64 Mi elements if nothing else ran).
+// 6.3 TB/s, reads alone 6.8), and for 8-bit moments nearly the vector units too (62 issue slots per
+// element, 106 us for 64 Mi elements if nothing else ran).
 // A plan's tensors are cut into tiles of 1024 elements, one workgroup each (64 Mi fp32: 4096 elements
 // by a loop took 346 us where one turn took 320).  A workgroup finds its tile's tensor through a table
 // with one entry per tile, so one launch serves any number of tensors; a single tensor's descriptor
@@ -245,8 +245,8 @@ __device__ __forceinline__ void adamw(float& p, float grad, float& m, float& v, 
 
 // fp32 moments: a workgroup takes one tile, 4 elements per lane.  Tiles in launch order: dealing each
 // XCD a contiguous eighth took 1287 instead of 1265 (256 Mi, bf16 with master), though 312 instead of
-// 322 for one 64 Mi buffer.  The kernel alone: 296 us for 64 Mi fp32 (6.35 TB/s), 1240 for the 256 Mi
-// (6.06), 95 for 291 ragged tensors' 624 MB.
+// 322 for one 64 Mi buffer.  The kernel alone: 296 to 305 us for 64 Mi fp32 (6.2 to 6.35 TB/s), 1240 to
+// 1253 for the 256 Mi (6.0), 95 to 97 for 291 ragged tensors' 624 MB.
 // fp32 square root and quotient are IEEE's: replacing both by the hardware's estimates gained nothing.
 template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kOptBlock) void k_adamw(const OptTensor* tensors,
@@ -383,7 +383,7 @@ __device__ __forceinline__ float uniform(float x, int lane) {
 }
 
 // A block's four elements per lane: decode, step, encode.  The vector units have 91 issue slots per
-// element while HBM delivers its 16 bytes; this takes 60 (counted in the assembly; with an IEEE
+// element while HBM delivers its 16 bytes; this takes 62 (counted in the assembly; with an IEEE
 // quotient in p's update the kernel took 170 us instead of 164).  The bytes are those of the documented
 // operations, each rounded to fp32.  Decoding is short where no byte stands for something not finite
 // and both old scales are below 2^15 (2^112 * scale is finite: one product per value).  The rest is
@@ -611,8 +611,8 @@ __device__ __forceinline__ w4 dwords_of(const Sixteen& x, bool odd) {
             __builtin_amdgcn_alignbit(x.d[2], x.d[1], 16), __builtin_amdgcn_alignbit(x.d[3], x.d[2], 16)};
 }
 
-// 2048 workgroups, 32 waves per CU: 64 Mi fp32 42 us (6.4 TB/s), 397 bf16 tensors of 100 M elements
-// 34 (5.9); fp32 sums instead of fp64 were no faster.
+// 2048 workgroups, 32 waves per CU: 64 Mi fp32 43 us (6.2 TB/s), 397 bf16 tensors of 100 M elements
+// 35 (5.7); fp32 sums instead of fp64 were no faster.
 // ALONE: the only workgroup, which finishes too.  KEEP: leave the gradients in the caches for the step
 // that reads them next: the norm alone takes 10 % longer, the two together 5 to 10 % less (128 MiB of
 // fp32 gradients 181 -> 162 us, 512 MiB 724 -> 702).  A plan of gradients alone has no step.

@@ -224,7 +224,8 @@ class AdamW:
     def grad_norm_(self, ctrl: Control, max_norm: float = 0.0, grad_scale: float = 1.0, bucket=None,
                    stream: int | None = None) -> None:
         """hydra_adamw_grad_norm: norm, clip factor and finite check of all gradients into ctrl, and
-        the next step's number.  max_norm 0: no clipping."""
+        the next step's number.  max_norm 0: no clipping.  stream: a raw handle; the tensors' ordering and
+        lifetime on another stream than torch's current one are the caller's."""
         h = self._h or self._closed()
         b = self._bucket_ptr(bucket) if self._bucket is not bucket else self._bucket_at
         if ctrl.index != self._index:

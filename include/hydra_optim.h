@@ -112,7 +112,8 @@ int hydra_adamw_destroy(hydra_adamw_t plan);
  * norm = |grad_scale| * sqrt(sum of all grad^2), summed in fp64 in an order fixed by the tensors'
  * lengths and the gradients' type, whatever the addresses: the same bits on every call and on every
  * rank that holds the same bits.  max_norm > 0 clips:
- * mult = grad_scale * min(1, max_norm / (norm + 1e-6)); 0: mult = grad_scale.  If the sum is not
+ * mult = grad_scale * min(1, max_norm / (norm + 1e-6)); 0: mult = grad_scale.  (Both are arguments: a
+ * captured graph keeps those of its capture.)  If the sum is not
  * finite, skip = 1 and skipped += 1; else step += 1 and the fields for that step are set.
  * workspace: hydra_adamw_workspace() bytes of device memory or more (none for a small plan: may be
  * NULL then), 8-byte aligned, needed until the call has run, and by graphs that hold it; its contents

@@ -112,7 +112,9 @@ class AdamW:
 
     Plans are made and closed while no thread captures a stream.  One that is dropped without close()
     waits with its device tables (88 bytes a tensor and 4 for 1024 elements) until the next one is made or
-    closed, so plans may be dropped at any time."""
+    closed, so plans may be dropped at any time.  close() waits for the device's work, dropping does not:
+    what a plan alone kept alive and used on another stream than its own follows torch's rule for such
+    tensors (record_stream, or close() first)."""
 
     def __init__(self, params, grads, m=None, v=None, *, master=None, m_scale=None, v_scale=None,
                  betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0,
